@@ -99,6 +99,28 @@ class CbmWalkStreamDev(C.Structure):
     ]
 
 
+class CbmNormBatch(C.Structure):
+    """Mirror of ``struct cbm_norm_batch`` (the rows of a batch of graphs)."""
+    _fields_ = [
+        ("samples", C.c_int32), ("max_len", C.c_int32), ("rows", C.c_int32), ("piece_rows", C.c_int32),
+        ("n_pieces", C.c_int32), ("reserved", C.c_int32),
+        ("ptr", C.c_void_p), ("pieces", C.c_void_p), ("piece_ptr", C.c_void_p),
+    ]
+
+
+class CbmOrthoItem(C.Structure):
+    """Mirror of ``struct cbm_ortho_item`` (one matrix of an orthogonalisation or optimiser step)."""
+    _fields_ = [
+        ("src", C.c_void_p), ("dst", C.c_void_p), ("weight", C.c_void_p), ("momentum", C.c_void_p),
+        ("rows", C.c_int32), ("cols", C.c_int32),
+        ("ld_src", C.c_int64), ("ld_dst", C.c_int64), ("ld_weight", C.c_int64), ("ld_momentum", C.c_int64),
+    ]
+
+
+CBM_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+CBM_LABELS_MAX_TOP = 32
+CBM_ORTHO_MAX_ITEMS = 24
+
 CBM_WALK_LOAD_ONLY = 63
 CBM_STREAM_LAST, CBM_STREAM_DUMMY, CBM_STREAM_COL_MASK = 0x40000000, 0x20000000, 0x1FFFFFFF
 CBM_STREAM_ROW_COST = 5
@@ -106,6 +128,7 @@ CBM_WALK_MAX_SLOTS = 31
 
 _P = C.c_void_p
 _I32, _I64 = C.c_int32, C.c_int64
+_F32 = C.c_float
 
 # name -> (restype, argtypes); the single list every symbol check iterates over
 HOST_SYMBOLS = {
@@ -160,6 +183,15 @@ HIP_SYMBOLS = {
     "cbm_spmm_update_tiled_f32": (C.c_int, [C.POINTER(CbmTilingDev), _P, _P, _P, _P, _P, _I32, _P, _P, _P, _I32, _I32, _I64,
                                             _I64, _I32, _P]),
     "csr_spmm_f32": (C.c_int, [_P, _P, _I64, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _P]),
+    "cbm_group_norm_workspace_floats": (C.c_int64, [_P, _I32, _I32, _I32, _I32]),
+    "cbm_group_norm_forward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _F32, _I32, _I32, _P]),
+    "cbm_group_norm_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _I32, _I32, _P]),
+    "cbm_label_scores_workspace_floats": (C.c_int64, [_I32, _I32, _I32]),
+    "cbm_label_scores": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _P]),
+    "cbm_label_scores_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I64, _I32, _P]),
+    "cbm_ortho_workspace_bytes": (C.c_int64, [_P, _I32]),
+    "cbm_orthogonalise": (C.c_int, [_P, _I32, _I32, _F32, _F32, _F32, _F32, _I32, _P, _P]),
+    "cbm_muon_step": (C.c_int, [_P, _I32, _F32, _F32, _F32, _I32, _I32, _F32, _F32, _F32, _F32, _P, _P]),
     "cbm_row_intersections_groups": (C.c_int, []),
     "cbm_row_intersections": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _I64, _P, _P]),
 }

@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -23,7 +24,7 @@ HOST_LIB = os.path.join(LIB_DIR, "libcbm_host.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_FLAGS = [
-    "-O3", "--offload-arch=gfx950", "-shared", "-fPIC", "-std=c++17",
+    "-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17",
     "-ffp-contract=off",                       # FMAs are written explicitly where they are meant
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
@@ -38,9 +39,17 @@ def _run(cmd):
     return out
 
 
+HIP_SOURCES = ["cbm_kernels.hip", "norm_kernels.hip", "label_kernels.hip", "ortho_kernels.hip"]
+
+
 def build_hip(verbose: bool = False) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
-    out = _run([HIPCC, *HIP_FLAGS, "-o", HIP_LIB, os.path.join(SRC_DIR, "cbm_kernels.hip")])
+    # one object per source, side by side, then the library
+    objects = [os.path.join(LIB_DIR, name.replace(".hip", ".o")) for name in HIP_SOURCES]
+    with ThreadPoolExecutor(len(HIP_SOURCES)) as pool:
+        outs = list(pool.map(lambda so: _run([HIPCC, *HIP_FLAGS, "-c", "-o", so[1], os.path.join(SRC_DIR, so[0])]),
+                             zip(HIP_SOURCES, objects)))
+    out = "\n".join(o for o in outs + [_run([HIPCC, *HIP_FLAGS, "-shared", "-o", HIP_LIB, *objects])] if o.strip())
     if verbose and out.strip():
         print(out)
     return HIP_LIB

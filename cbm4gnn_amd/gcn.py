@@ -30,6 +30,11 @@ the multiply:
   next call of the same layer.  A backward that would read an overwritten buffer raises: the layer
   counts its forward calls and bumps the buffer's autograd version, so ``forward, forward, backward
   of the first`` is an error, never a wrong gradient (``fused=False`` allocates per call instead).
+
+Around the layers: ``CBMGCNLayer(norm=GroupNorm(...), graphs=GraphBatch(...))`` normalises the aggregated
+features per graph of a batch, with an activation; ``TwoLayerGCN.loss`` and ``.answer`` score the logits
+(``labels.label_log_probs``); ``optimizers`` and ``train_step`` update the weights (``optim.Muon`` for the
+matrices, Adam for what is not one).
 """
 from __future__ import annotations
 
@@ -42,8 +47,12 @@ from torch import nn
 
 from . import _lib
 from .cbm import DEFAULT_BATCH_ROWS, CBMMatmul, _ld, _ptr, _wants_workspace, cbm_matrix, csr_spmm, relayout_slabs, schedule_rows
+from .labels import LabelScores, label_log_probs
+from .norm import GraphBatch, GroupNorm
+from .optim import Muon
 
-__all__ = ["CBMGCNLayer", "CSRGCNLayer", "TwoLayerGCN", "build_operator", "csr_operator", "CSRMatmul", "tuned_gemms"]
+__all__ = ["CBMGCNLayer", "CSRGCNLayer", "TwoLayerGCN", "build_operator", "csr_operator", "CSRMatmul", "tuned_gemms",
+           "optimizers", "train_step"]
 
 
 @contextlib.contextmanager
@@ -134,12 +143,22 @@ class _FusedGCNLayer(torch.autograd.Function):
 
 
 class CBMGCNLayer(nn.Module):
-    """``x -> [relu](A_hat (x W^T))``: the reference's GCN layer (``cbm_gcn.py:27-41``) with the
+    """``x -> [norm]([relu](A_hat (x W^T)))``: the reference's GCN layer (``cbm_gcn.py:27-41``) with the
     activation that follows it in the benchmark model optionally folded in (``relu=True``).
-    ``fused=False`` is the plain composition Linear -> ``CBMMatmul`` (-> ``relu``)."""
+    ``fused=False`` is the plain composition Linear -> ``CBMMatmul`` (-> ``relu``).  ``norm``: a ``GroupNorm`` of
+    the output channels (its activation takes the ReLU's place), over all nodes or, with ``graphs``, over the
+    nodes of each graph of a block-diagonal operator."""
 
-    def __init__(self, in_channels: int, out_channels: int, operator: cbm_matrix, fused: bool = True, relu: bool = False):
+    def __init__(self, in_channels: int, out_channels: int, operator: cbm_matrix, fused: bool = True, relu: bool = False,
+                 norm: GroupNorm | None = None, graphs: GraphBatch | None = None):
         super().__init__()
+        if norm is not None and norm.channels != out_channels:
+            raise ValueError(f"norm has {norm.channels} channels, the layer {out_channels}")
+        if graphs is not None and norm is None:
+            raise ValueError("graphs are the norm's: give a norm")
+        if graphs is not None and graphs.n_nodes != operator.num_rows:
+            raise ValueError(f"the batch has {graphs.n_nodes} nodes, the operator {operator.num_rows}")
+        self.norm, self.graphs = norm, graphs
         self.lin = nn.Linear(in_channels, out_channels, bias=False)
         nn.init.xavier_uniform_(self.lin.weight)            # 'glorot'
         self.cached_a_t = operator
@@ -177,9 +196,11 @@ class CBMGCNLayer(nn.Module):
 
     def forward(self, x, edge_index=None):
         if self.fused and x.is_cuda:
-            return _FusedGCNLayer.apply(x, self.lin.weight, self)
-        y = CBMMatmul.apply(self.lin(x), self.cached_a_t, self.cached_a_t.col_multiplier is not None)
-        return y.relu() if self.relu else y
+            y = _FusedGCNLayer.apply(x, self.lin.weight, self)
+        else:
+            y = CBMMatmul.apply(self.lin(x), self.cached_a_t, self.cached_a_t.col_multiplier is not None)
+            y = y.relu() if self.relu else y
+        return y if self.norm is None else self.norm(y, self.graphs)
 
 
 class CSRMatmul(torch.autograd.Function):
@@ -240,3 +261,34 @@ class TwoLayerGCN(nn.Module):
     def forward(self, x, edge_index=None):
         h = self.first_layer(x, edge_index)
         return self.last_layer(h.relu() if self.relu_between else h, edge_index)
+
+    def loss(self, x, labels, ignore_index: int = -100):
+        """Mean negative log probability of the labels over the nodes that have one (0 where none has)."""
+        r = label_log_probs(self(x), labels, ignore_index=ignore_index)
+        return -r.logp.sum() / (labels != ignore_index).sum().clamp(min=1)
+
+    @torch.no_grad()
+    def answer(self, x, top: int = 1) -> LabelScores:
+        """The ``top`` likeliest classes of every node, their log probabilities and the entropy of the node's
+        distribution."""
+        return label_log_probs(self(x), entropy=True, top=top)
+
+
+def optimizers(model: nn.Module, lr: float = 0.02, weight_decay: float = 0.0, vector_lr: float = 1e-3):
+    """``Muon`` over the matrices of ``model`` and, where it has other parameters (a norm's weight and bias), Adam
+    over those."""
+    params = [p for p in model.parameters() if p.requires_grad]
+    matrices, others = [p for p in params if p.dim() == 2], [p for p in params if p.dim() != 2]
+    out = [Muon(matrices, lr=lr, weight_decay=weight_decay)] if matrices else []
+    return out + ([torch.optim.Adam(others, lr=vector_lr)] if others else [])
+
+
+def train_step(model: TwoLayerGCN, x, labels, opts, ignore_index: int = -100):
+    """One step: loss, gradients, update by each of ``opts``.  Returns the loss (a tensor, nothing waits for it)."""
+    for o in opts:
+        o.zero_grad(set_to_none=True)
+    loss = model.loss(x, labels, ignore_index)
+    loss.backward()
+    for o in opts:
+        o.step()
+    return loss.detach()

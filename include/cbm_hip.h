@@ -609,6 +609,85 @@ int csr_spmm_f32(const int32_t* rowptr_dev, const int32_t* col_dev, int64_t nnz,
                  const int32_t* row_sched_dev, const float* X_dev, float* Y_dev, float* workspace_dev,
                  int32_t flags, int32_t n, int32_t d, int64_t ldx, int64_t ldy, void* stream);
 
+/* -------------------------------------------------------------------------------------------------
+ * Dense operators of a GCN step around the aggregation: normalisation between layers, scores of the
+ * labels, update of the weights.  The reference leaves all three to torch (its benchmark model has a
+ * ReLU between the layers and nothing else, benchmark/parallel/benchmark_gcn_cpu.py:62-89).  Same
+ * conventions as above: device pointers, row strides in elements, caller-owned workspace, no
+ * allocation, no synchronisation, a status for an answer.  Sums and statistics are fp32.
+ * ------------------------------------------------------------------------------------------------- */
+enum { CBM_DTYPE_F32 = 0, CBM_DTYPE_BF16 = 1, CBM_DTYPE_F16 = 2 };   /* elements of X, Y, logits, matrices */
+enum { CBM_ACT_NONE = 0, CBM_ACT_RELU = 1, CBM_ACT_SILU = 2 };
+
+/* The rows of a batch of graphs.  Equal lengths (one graph: samples = 1): ptr = NULL, max_len rows each.
+ * Ragged: ptr (device, samples + 1 row offsets, ptr[0] = 0, ptr[samples] = rows, ascending) and the rows cut
+ * into pieces of at most piece_rows, no piece across two graphs: pieces (device, n_pieces times {graph, first
+ * row, rows, 0}, by graph and row) and piece_ptr (device, samples + 1: first piece of each graph).  The
+ * kernels index with these arrays as they are. */
+typedef struct cbm_norm_batch {
+    int32_t samples, max_len, rows, piece_rows, n_pieces, reserved;
+    const int32_t* ptr;
+    const int32_t* pieces;
+    const int32_t* piece_ptr;
+} cbm_norm_batch;
+
+/* Y = act(group_norm(X)) for X, Y [rows, C] of dtype, statistics per graph and group of C / groups channels;
+ * weight and bias (fp32 [C]) may be NULL (1 and 0).  mean, rstd: fp32 [samples, groups] for the backward, both
+ * or neither.  workspace: cbm_group_norm_workspace_floats(.., backward = 0) floats, may be NULL if that is 0. */
+int64_t cbm_group_norm_workspace_floats(const cbm_norm_batch* batch, int32_t C, int32_t groups, int32_t dtype, int32_t backward);
+int cbm_group_norm_forward(const cbm_norm_batch* batch, const void* X_dev, void* Y_dev, const float* weight_dev,
+                           const float* bias_dev, float* mean_dev, float* rstd_dev, float* workspace_dev, int32_t C,
+                           int32_t groups, int64_t ldx, int64_t ldy, float eps, int32_t act, int32_t dtype, void* stream);
+/* Gradients for DY [rows, C]: DX (nullable), dweight and dbias (nullable; zero where the batch has no rows).
+ * DX may be DY.  workspace: cbm_group_norm_workspace_floats(.., backward = 1) floats. */
+int cbm_group_norm_backward(const cbm_norm_batch* batch, const void* X_dev, const void* DY_dev, void* DX_dev,
+                            const float* weight_dev, const float* bias_dev, const float* mean_dev, const float* rstd_dev,
+                            float* dweight_dev, float* dbias_dev, float* workspace_dev, int32_t C, int32_t groups,
+                            int64_t ldx, int64_t ldg, int64_t ldd, int32_t act, int32_t dtype, void* stream);
+
+/* Scores of given labels under softmax(logits), logits [rows, classes] of dtype:
+ *   logp    [rows] fp32 (nullable)       log probability of labels[row]; 0 where it is ignore_index, NaN where it
+ *                                        is any other value outside [0, classes)
+ *   entropy [rows] fp32 (nullable)       -sum p log p
+ *   top_logp, top_index [rows, top]      the `top` (0 .. CBM_LABELS_MAX_TOP) largest logits of the row, descending, equal
+ *           fp32, int64                  ones by ascending index, NaN before everything: their log probabilities, places
+ *   stats   [rows, 2] fp32 (nullable)    what the backward needs: {max, log sum exp(logit - max)}
+ * A row of -inf alone has log probabilities -inf and entropy 0; a NaN or +inf in a row makes its scores NaN.
+ * workspace: cbm_label_scores_workspace_floats() floats, may be NULL if that is 0. */
+enum { CBM_LABELS_MAX_TOP = 32 };
+int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t top);
+int cbm_label_scores(const void* logits_dev, const int64_t* labels_dev, float* logp_dev, float* entropy_dev, float* top_logp_dev,
+                     int64_t* top_index_dev, float* stats_dev, float* workspace_dev, int32_t rows, int32_t classes, int32_t top,
+                     int64_t ld, int64_t ignore_index, int32_t dtype, void* stream);
+/* grad [rows, classes] of dtype, from the gradients of logp, entropy (which then is given too) and top_logp, each nullable. */
+int cbm_label_scores_backward(const void* logits_dev, const int64_t* labels_dev, const float* stats_dev, const float* entropy_dev,
+                              const int64_t* top_index_dev, const float* g_logp_dev, const float* g_entropy_dev,
+                              const float* g_top_dev, void* grad_dev, int32_t rows, int32_t classes, int32_t top, int64_t ld,
+                              int64_t ldg, int64_t ignore_index, int32_t dtype, void* stream);
+
+/* Newton-Schulz orthogonalisation of matrices G [rows, cols], and the optimiser step around it:
+ *   X = G / (|G|_F + eps);  `steps` times: X = a X + (b A + c A A) X with A = X X^T  (taken on the shorter side)
+ * A list of matrices of any shapes shares its launches; up to CBM_ORTHO_MAX_ITEMS go together, longer lists in
+ * turns.  The products run on the matrix cores with every operand split into two halves of 11 bits (see
+ * ortho_kernels.hip), sums in fp32; an item of zeros gives zeros. */
+enum { CBM_ORTHO_MAX_ITEMS = 24 };
+typedef struct cbm_ortho_item {
+    const void* src;         /* G [rows, cols], dtype; in cbm_muon_step the gradient, fp32            */
+    void* dst;               /* cbm_orthogonalise: result [rows, cols], dtype, not src                 */
+    float* weight;           /* cbm_muon_step: fp32 weight, updated                                    */
+    float* momentum;         /* cbm_muon_step: fp32 momentum buffer, updated                           */
+    int32_t rows, cols;
+    int64_t ld_src, ld_dst, ld_weight, ld_momentum;
+} cbm_ortho_item;
+
+int64_t cbm_ortho_workspace_bytes(const cbm_ortho_item* items, int32_t n_items);
+int cbm_orthogonalise(const cbm_ortho_item* items, int32_t n_items, int32_t steps, float a, float b, float c, float eps,
+                      int32_t dtype, void* workspace_dev, void* stream);
+/* momentum = mu momentum + G;  U = G + mu momentum (nesterov) or momentum;  O = orthogonalised U;
+ * weight = (1 - lr decay) weight - lr sqrt(max(1, rows / cols)) O */
+int cbm_muon_step(const cbm_ortho_item* items, int32_t n_items, float lr, float mu, float decay, int32_t nesterov, int32_t steps,
+                  float a, float b, float c, float eps, void* workspace_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
