@@ -104,7 +104,7 @@ class CbmNormBatch(C.Structure):
     _fields_ = [
         ("samples", C.c_int32), ("max_len", C.c_int32), ("rows", C.c_int32), ("piece_rows", C.c_int32),
         ("n_pieces", C.c_int32), ("reserved", C.c_int32),
-        ("ptr", C.c_void_p), ("pieces", C.c_void_p), ("piece_ptr", C.c_void_p),
+        ("ptr", C.c_void_p), ("pieces", C.c_void_p), ("piece_ptr", C.c_void_p), ("order", C.c_void_p),
     ]
 
 

@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/cbm_hip.h"
 
 namespace cbm_dense {
@@ -16,6 +18,43 @@ constexpr int kWave = 64;
 
 template <typename T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[V]; };
+
+// V elements as they lie in memory, held as 32-bit words (as elements, two-byte types would take a register each).
+template <typename T, int V>
+struct Raw {
+    static constexpr int kWords = (V * sizeof(T) + 3) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)))));
+    }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T* __restrict__ p) {
+    Raw<T, V> r;
+    if constexpr (V * sizeof(T) < 4) {
+        r.w[0] = __builtin_bit_cast(uint16_t, *p);
+    } else {
+        struct __attribute__((packed, aligned(sizeof(T)))) Words { uint32_t w[Raw<T, V>::kWords]; };
+        const Words t = *reinterpret_cast<const Words*>(p);
+#pragma unroll
+        for (int i = 0; i < Raw<T, V>::kWords; ++i) r.w[i] = t.w[i];
+    }
+    return r;
+}
+
+// Makes a value opaque to the compiler: what was computed from it before is computed again, not kept in registers.
+__device__ __forceinline__ void forget(uint32_t& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void forget(int& v) { asm volatile("" : "+v"(v)); }
+template <typename T, int V, int N>
+__device__ __forceinline__ void forget(Raw<T, V> (&raw)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int i = 0; i < Raw<T, V>::kWords; ++i) forget(raw[k].w[i]);
+}
 
 template <typename T, int V>
 __device__ __forceinline__ void load_as_f32(const T* __restrict__ p, float (&out)[V]) {

@@ -622,13 +622,15 @@ enum { CBM_ACT_NONE = 0, CBM_ACT_RELU = 1, CBM_ACT_SILU = 2 };
 /* The rows of a batch of graphs.  Equal lengths (one graph: samples = 1): ptr = NULL, max_len rows each.
  * Ragged: ptr (device, samples + 1 row offsets, ptr[0] = 0, ptr[samples] = rows, ascending) and the rows cut
  * into pieces of at most piece_rows, no piece across two graphs: pieces (device, n_pieces times {graph, first
- * row, rows, 0}, by graph and row) and piece_ptr (device, samples + 1: first piece of each graph).  The
- * kernels index with these arrays as they are. */
+ * row, rows, 0}, by graph and row) and piece_ptr (device, samples + 1: first piece of each graph).  order
+ * (device, samples, may be NULL): the graphs in the order they are begun in, longest first.  The kernels index
+ * with these arrays as they are. */
 typedef struct cbm_norm_batch {
     int32_t samples, max_len, rows, piece_rows, n_pieces, reserved;
     const int32_t* ptr;
     const int32_t* pieces;
     const int32_t* piece_ptr;
+    const int32_t* order;
 } cbm_norm_batch;
 
 /* Y = act(group_norm(X)) for X, Y [rows, C] of dtype, statistics per graph and group of C / groups channels;
