@@ -119,6 +119,7 @@ class CbmOrthoItem(C.Structure):
 
 CBM_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
 CBM_LABELS_MAX_TOP = 32
+CBM_LABELS_MAX_CLASSES = 64 * 1024 * 8 * 4
 CBM_ORTHO_MAX_ITEMS = 24
 
 CBM_WALK_LOAD_ONLY = 63
@@ -186,7 +187,7 @@ HIP_SYMBOLS = {
     "cbm_group_norm_workspace_floats": (C.c_int64, [_P, _I32, _I32, _I32, _I32]),
     "cbm_group_norm_forward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _F32, _I32, _I32, _P]),
     "cbm_group_norm_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _I32, _I32, _P]),
-    "cbm_label_scores_workspace_floats": (C.c_int64, [_I32, _I32, _I32]),
+    "cbm_label_scores_workspace_floats": (C.c_int64, [_I32, _I32, _I32, _I32]),
     "cbm_label_scores": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _P]),
     "cbm_label_scores_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I64, _I32, _P]),
     "cbm_ortho_workspace_bytes": (C.c_int64, [_P, _I32]),

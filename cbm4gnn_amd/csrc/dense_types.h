@@ -31,6 +31,21 @@ struct Raw {
     }
 };
 
+// Makes the first n elements -inf.
+template <typename T, int V>
+__device__ __forceinline__ void lowest(Raw<T, V>& r, int n) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if (i >= n) continue;
+        if constexpr (sizeof(T) == 4) {
+            r.w[i] = 0xff800000u;
+        } else {
+            constexpr uint32_t kBits = std::is_same<T, __bf16>::value ? 0xff80u : 0xfc00u;
+            r.w[i / 2] = i % 2 ? (r.w[i / 2] & 0xffffu) | kBits << 16 : (r.w[i / 2] & 0xffff0000u) | kBits;
+        }
+    }
+}
+
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> load_raw(const T* __restrict__ p) {
     Raw<T, V> r;
@@ -72,23 +87,49 @@ __device__ __forceinline__ void store_from_f32(T* __restrict__ p, const float (&
     *reinterpret_cast<Pack<T, V>*>(p) = t;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// One step of a reduction over groups of 2 O lanes, where all lanes of each half already agree: the values of both halves.
+// Data-parallel moves and lane swaps, one vector instruction each (a shuffle goes through the LDS unit instead).
+struct Halves { uint32_t a, b; };
+template <int O>
+__device__ __forceinline__ Halves halves(uint32_t v) {
+    if constexpr (O == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return {static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1])};
+    } else if constexpr (O == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return {static_cast<uint32_t>(r[0]), static_cast<uint32_t>(r[1])};
+    } else {
+        // lane ^ 1, lane ^ 2 within four; mirrors of half rows and rows, which agree within their halves
+        constexpr int kCtrl = O == 1 ? 0xB1 : O == 2 ? 0x4E : O == 4 ? 0x141 : 0x140;
+        static_assert(O == 1 || O == 2 || O == 4 || O == 8, "steps of a wavefront");
+        return {v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), kCtrl, 0xf, 0xf, true))};
+    }
 }
 
-// Sum over the workgroup, the same value in every thread, in a fixed order.  lds: one float per wavefront.
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-    v = wave_sum(v);
-    const int waves = (blockDim.x + kWave - 1) / kWave;
-    if (waves == 1) return v;
-    __syncthreads();                                       // the last use of lds is over
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float s = 0.f;
-    for (int w = 0; w < waves; ++w) s += lds[w];
-    return s;
+// Reduces over groups of L lanes by step(halves of the same O for whatever the caller holds), O = 1, 2, .. L / 2.
+template <int L, int O = 1, typename Step>
+__device__ __forceinline__ void reduce_lanes(Step step) {
+    if constexpr (O < L) {
+        step(std::integral_constant<int, O>());
+        reduce_lanes<L, 2 * O>(step);
+    }
+}
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+    reduce_lanes<L>([&](auto o) {
+        const Halves h = halves<decltype(o)::value>(__float_as_uint(v));
+        v = __uint_as_float(h.a) + __uint_as_float(h.b);
+    });
+    return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+    reduce_lanes<L>([&](auto o) {
+        const Halves h = halves<decltype(o)::value>(__float_as_uint(v));
+        v = fmaxf(__uint_as_float(h.a), __uint_as_float(h.b));
+    });
+    return v;
 }
 
 inline int check_launch() { return hipGetLastError() == hipSuccess ? CBM_OK : CBM_ERR_LAUNCH; }

@@ -6,16 +6,23 @@
 //
 // m and log S are kept apart (not summed into one float), so logits far from zero cost no digits.
 //
-// One pass over the logits serves all three: running maximum, sum and weighted sum.  Reading the logits bounds the
-// forward, reading them and writing the gradient the backward.
-//   narrow   up to 1024 classes: L lanes hold a row in registers (at most 16 values each), 64 / L rows per wavefront;
-//   wide     a workgroup per row, 16-byte loads; with few rows the columns are split over workgroups whose partial
-//            results a second launch joins.
+// A row is read once and stays in registers for its maximum, its sums and its likeliest classes.  Reading the logits
+// bounds the forward, reading them and writing the gradient the backward; with some ten vector instructions a value
+// (the exponential alone costs four issue slots) arithmetic is not far behind.
+//   narrow   up to 1024 classes: 4 to 64 lanes hold a row in vectors of 16 bytes, up to 16 rows per wavefront;
+//   wide     a workgroup per row.  Rows longer than a workgroup's registers, and long rows that are few, are split
+//            over workgroups whose partial results a second launch joins.
+// Measured (one MI355X, kernel times): 232 965 x 41 fp32: scores 9.0 us (4.4 TB/s), gradient 17.2 us (4.5 TB/s);
+// 12 000 x 41 fp32 with entropy and 5 classes: 4.8 us;  2 049 x 32 003 bf16 with entropy and 8 classes: 54 us (2.4 TB/s,
+// bound by its 16 vector instructions a value), gradient 45 us (5.8 TB/s);  1 x 100 000 fp32 with entropy and 10 classes:
+// 7.8 + 5.6 us, two launches' latency.
+// The last vector of a row begins where it still fits and overlaps the one before, whose values it ignores.
+//
 // Likeliest classes order by (value, lowest index): value and index make ONE 64-bit key, so no two are equal and the
 // answer does not depend on who looks at what.  Narrow rows take `top` maxima out of registers.  Wide rows first
-// find a bound that at least `top` keys reach (the `top`-th largest of 128 maxima of disjoint parts of the row),
-// then collect the few keys above it into LDS and rank them by counting; a row that crowds more than the list holds
-// into few parts takes one more pass per class instead.
+// find a bound that at least `top` values reach (the `top`-th largest of the maxima of 128 disjoint parts), then
+// collect the few values above it into LDS and rank them by counting; a row that crowds more than the list holds
+// above its bound takes `top` maxima instead.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -29,8 +36,7 @@ using namespace cbm_dense;
 using key_t = unsigned long long;
 
 constexpr int kMaxTop = CBM_LABELS_MAX_TOP;
-constexpr int kNarrowThreads = 256;
-constexpr int kWideThreads = 1024;
+constexpr int kThreads = 256;
 constexpr int kParts = 128;                // disjoint parts of a wide row whose maxima bound its likeliest classes
 constexpr int kList = 2048;                // candidates a wide row keeps
 constexpr float kInf = __builtin_inff();
@@ -41,20 +47,24 @@ __device__ __forceinline__ unsigned order_of(float v) {
     if (v != v) return 0xffc00000u;
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float value_of(unsigned o) {
-    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
-}
+__device__ __forceinline__ float value_of(unsigned o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ key_t key_of(unsigned order, unsigned index) {
     return (static_cast<key_t>(order) << 32) | (0xffffffffu - index);
 }
 __device__ __forceinline__ unsigned index_of(key_t k) { return 0xffffffffu - static_cast<unsigned>(k); }
 
-__device__ __forceinline__ key_t shfl_xor_key(key_t k, int o) {
-    const unsigned lo = __shfl_xor(static_cast<unsigned>(k), o), hi = __shfl_xor(static_cast<unsigned>(k >> 32), o);
-    return (static_cast<key_t>(hi) << 32) | lo;
+template <int L>
+__device__ __forceinline__ key_t lanes_max_key(key_t k) {
+    reduce_lanes<L>([&](auto o) {
+        constexpr int O = decltype(o)::value;
+        const Halves lo = halves<O>(static_cast<uint32_t>(k)), hi = halves<O>(static_cast<uint32_t>(k >> 32));
+        const key_t a = (static_cast<key_t>(hi.a) << 32) | lo.a, b = (static_cast<key_t>(hi.b) << 32) | lo.b;
+        k = a > b ? a : b;
+    });
+    return k;
 }
 
-// Running softmax sums: m the maximum, s = sum exp(z - m), t = sum exp(z - m) (z - m).
+// Softmax sums: m the maximum, s = sum exp(z - m), t = sum exp(z - m) (z - m).
 struct Sums { float m, s, t; };
 
 __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
@@ -65,18 +75,24 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
     return {m, a.s * fa + b.s * fb, ta + tb};
 }
 
-// Takes one value into sums whose maximum already covers it; base = m, or 0 while m is -inf.
+template <int L>
+__device__ __forceinline__ Sums lanes_join(Sums S) {
+    reduce_lanes<L>([&](auto o) {
+        constexpr int O = decltype(o)::value;
+        const Halves m = halves<O>(__float_as_uint(S.m)), s = halves<O>(__float_as_uint(S.s)), t = halves<O>(__float_as_uint(S.t));
+        S = join(Sums{__uint_as_float(m.a), __uint_as_float(s.a), __uint_as_float(t.a)},
+                 Sums{__uint_as_float(m.b), __uint_as_float(s.b), __uint_as_float(t.b)});
+    });
+    return S;
+}
+
+// Takes one value into sums whose maximum already covers it; base = m, or 0 while m is -inf.  The exponential of
+// anything under -200 is 0, so the product's other factor may stop there: exp(-inf) (-inf) counts nothing.
+template <bool T>
 __device__ __forceinline__ void take(Sums& S, float v, float base) {
     const float d = v - base, e = __expf(d);
     S.s += e;
-    S.t += e > 0.f ? e * d : 0.f;                          // exp(-inf) (-inf) counts nothing
-}
-
-template <int L>
-__device__ __forceinline__ Sums join_lanes(Sums S) {
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) S = join(S, Sums{__shfl_xor(S.m, o), __shfl_xor(S.s, o), __shfl_xor(S.t, o)});
-    return S;
+    if constexpr (T) S.t = __builtin_fmaf(e, fmaxf(d, -200.f), S.t);
 }
 
 struct Outputs {
@@ -101,7 +117,7 @@ __device__ __forceinline__ Final finish(const Sums& S) {
 
 template <typename T>
 __device__ __forceinline__ void write_scores(const Outputs& O, const T* __restrict__ row, int64_t r, const Final& F) {
-    if (O.stats) { O.stats[2 * r] = F.m; O.stats[2 * r + 1] = F.log_s; }
+    if (O.stats) *reinterpret_cast<float2*>(O.stats + 2 * r) = make_float2(F.m, F.log_s);
     if (O.entropy) O.entropy[r] = F.h;
     if (O.logp) {
         const int64_t y = O.labels[r];
@@ -117,53 +133,68 @@ __device__ __forceinline__ void write_top(const Outputs& O, int64_t r, int i, ke
     O.top_index[r * O.top + i] = index_of(k);
 }
 
+// Vector i of the columns [.., hi): its columns at .. at + V - 1, of which those from `first` on are its own.
+struct Place { int at, first; };
+template <int V>
+__device__ __forceinline__ Place place_of(int first, int hi) { return {min(first, hi - V), first}; }
+
 // ---------------------------------------------------------------------------------------------
-// narrow rows
+// narrow rows: vector j of lane l covers the columns (l + L j) V ..; only the last j meets the row's end
 // ---------------------------------------------------------------------------------------------
-template <typename T, int L, int NV>
-__global__ __launch_bounds__(kNarrowThreads) void label_scores_narrow(const T* __restrict__ Z, int64_t ld, int rows, Outputs O) {
+template <typename T, int V, int L, int NV>
+__device__ __forceinline__ void load_narrow(const T* __restrict__ row, int lane, int classes, float otherwise, float (&v)[NV][V]) {
+    Raw<T, V> raw[NV];
+    const Place last = place_of<V>((lane + L * (NV - 1)) * V, classes);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) raw[j] = load_raw<T, V>(row + (j < NV - 1 ? (lane + L * j) * V : last.at));
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = j < NV - 1 || last.at + i >= last.first ? raw[j][i] : otherwise;
+}
+
+// ALL: entropy or likeliest classes are asked for too
+template <typename T, int V, int L, int NV, bool ALL>
+__global__ __launch_bounds__(kThreads) void label_scores_narrow(const T* __restrict__ Z, int64_t ld, int rows, Outputs O) {
     const int lane = threadIdx.x % L;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / L) + threadIdx.x / L;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
     const T* row = Z + min(r, static_cast<int64_t>(rows - 1)) * ld;
-    float v[NV];
+    float v[NV][V];
+    load_narrow<T, V, L, NV>(row, lane, O.classes, -kInf, v);
     Sums S{-kInf, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = lane + L * j;
-        v[j] = c < O.classes ? static_cast<float>(row[c]) : -kInf;
-    }
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int j = 0; j < NV; ++j) S.m = fmaxf(S.m, v[j]);
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) S.m = fmaxf(S.m, __shfl_xor(S.m, o));
+        for (int i = 0; i < V; ++i) S.m = fmaxf(S.m, v[j][i]);
+    S.m = lanes_max<L>(S.m);
     const float base = S.m == -kInf ? 0.f : S.m;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) take(S, v[j], base);
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) {
-        S.s += __shfl_xor(S.s, o);
-        S.t += __shfl_xor(S.t, o);
-    }
+        for (int i = 0; i < V; ++i) take<ALL>(S, v[j][i], base);
+    S.s = lanes_sum<L>(S.s);
+    if constexpr (ALL) S.t = lanes_sum<L>(S.t);
     const Final F = finish(S);
     const bool mine = r < rows && lane == 0;
     if (mine) write_scores<T>(O, row, r, F);
-    unsigned taken = 0;
-    for (int i = 0; i < O.top; ++i) {
-        unsigned best = 0, at = 0;
+    if constexpr (ALL) {
+        const Place last = place_of<V>((lane + L * (NV - 1)) * V, O.classes);
+        unsigned taken = 0;
+        for (int i = 0; i < O.top; ++i) {
+            unsigned best = 0, at = 0, bit = 0;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const unsigned c = lane + L * j;
-            const unsigned o = c < static_cast<unsigned>(O.classes) && !(taken >> j & 1u) ? order_of(v[j]) : 0u;
-            if (o > best) { best = o; at = c; }
-        }
-        key_t k = best ? key_of(best, at) : 0;
+            for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) {
-            const key_t other = shfl_xor_key(k, o);
-            k = other > k ? other : k;
+                for (int e = 0; e < V; ++e) {
+                    const unsigned b = 1u << (j * V + e), c = (j < NV - 1 ? (lane + L * j) * V : last.at) + e;
+                    const bool own = j < NV - 1 || last.at + e >= last.first;
+                    const unsigned o = own && !(taken & b) ? order_of(v[j][e]) : 0u;
+                    if (o > best) { best = o; at = c; bit = b; }
+                }
+            const key_t mine_k = best ? key_of(best, at) : 0, k = lanes_max_key<L>(mine_k);
+            if (best && k == mine_k) taken |= bit;
+            if (mine) write_top(O, r, i, k, F);
         }
-        if (best && index_of(k) == at) taken |= 1u << ((at - lane) / L);
-        if (mine) write_top(O, r, i, k, F);
     }
 }
 
@@ -179,21 +210,20 @@ struct Grads {
     int classes, top;
 };
 
-// What a row's gradient needs: dz_j = -p_j (all + gh (log p_j + h)) + gl [j = label] (+ the likeliest classes')
+// What a row's gradient needs: dz_j = -p_j (all + gh (log p_j + h)) + gl [j = label] (+ the likeliest classes').
 // A row of -inf alone has no gradient.
 struct RowGrad { float m, log_s, h, gl, gh, all; int label; bool any; };
 __device__ __forceinline__ RowGrad row_grad(const Grads& G, int64_t r) {
-    RowGrad R{G.stats[2 * r], G.stats[2 * r + 1], 0.f, 0.f, 0.f, 0.f, -1, true};
-    if (R.log_s == kInf) {
-        R.any = false;
-        return R;
-    }
+    const float2 st = *reinterpret_cast<const float2*>(G.stats + 2 * r);
+    RowGrad R{st.x, st.y, 0.f, 0.f, 0.f, 0.f, -1, st.y != kInf};
+    if (!R.any) return R;
     if (G.g_entropy) { R.gh = G.g_entropy[r]; R.h = G.entropy[r]; }
     if (G.g_logp) {
         const int64_t y = G.labels[r];
+        const float g = G.g_logp[r];
         if (y != G.ignore_index) {
             const bool in = y >= 0 && y < G.classes;
-            R.gl = in ? G.g_logp[r] : __builtin_nanf("");
+            R.gl = in ? g : __builtin_nanf("");
             R.label = in ? static_cast<int>(y) : -1;
         }
     }
@@ -202,166 +232,194 @@ __device__ __forceinline__ RowGrad row_grad(const Grads& G, int64_t r) {
         for (int i = 0; i < G.top; ++i) R.all += G.g_top[r * G.top + i];
     return R;
 }
+template <bool H>
 __device__ __forceinline__ float grad_of(const RowGrad& R, float z, int c) {
     const float lp = (z - R.m) - R.log_s, p = __expf(lp);
     // p = 0: nothing, also where log p is -inf; a NaN goes through
-    const float inner = p == 0.f ? R.all : __builtin_fmaf(R.gh, lp + R.h, R.all);
-    return (c == R.label ? R.gl : 0.f) - p * inner;
+    const float inner = H ? __builtin_fmaf(R.gh, (p == 0.f ? 0.f : lp) + R.h, R.all) : R.all;
+    return __builtin_fmaf(-p, inner, c == R.label ? R.gl : 0.f);
 }
 
-template <typename T, int L, int NV>
-__global__ __launch_bounds__(kNarrowThreads) void label_grads_narrow(const T* __restrict__ Z, T* __restrict__ D, int64_t ld, int64_t ldg,
-                                                                     int rows, Grads G) {
+template <typename T, int V, int L, int NV>
+__global__ __launch_bounds__(kThreads) void label_grads_narrow(const T* __restrict__ Z, T* __restrict__ D, int64_t ld, int64_t ldg,
+                                                               int rows, Grads G) {
     const int lane = threadIdx.x % L;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * (kNarrowThreads / L) + threadIdx.x / L;
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * (kThreads / L) + threadIdx.x / L;
     if (r >= rows) return;
-    const T* row = Z + r * ld;
-    float v[NV];
+    float v[NV][V];
+    load_narrow<T, V, L, NV>(Z + r * ld, lane, G.classes, 0.f, v);
+    const RowGrad R = row_grad(G, r);
+    // the last vector's overlap belongs to a neighbour; both write the same bits there
+    const Place last = place_of<V>((lane + L * (NV - 1)) * V, G.classes);
+    T* out = D + r * ldg;
+    const bool likeliest = G.g_top && R.any;
+    float z[V];
+    if (last.at < last.first) {                            // the overlap's values, which load_narrow left out
+        const Raw<T, V> raw = load_raw<T, V>(Z + r * ld + last.at);
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = raw[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) z[i] = v[NV - 1][i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[NV - 1][i] = z[i];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int c = lane + L * j;
-        v[j] = c < G.classes ? static_cast<float>(row[c]) : 0.f;
+        const int at = j < NV - 1 ? (lane + L * j) * V : last.at;
+        if (G.g_entropy) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j][i] = grad_of<true>(R, v[j][i], at + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[j][i] = grad_of<false>(R, v[j][i], at + i);
+        }
     }
-    const RowGrad R = row_grad(G, r);
+    if (likeliest)
+        for (int k = 0; k < G.top; ++k) {
+            const int64_t c = G.top_index[r * G.top + k];
+            const float g = G.g_top[r * G.top + k];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = grad_of(R, v[j], lane + L * j);
-    if (G.g_top && R.any)
-        for (int i = 0; i < G.top; ++i) {
-            const int64_t at = G.top_index[r * G.top + i];
-            const float g = G.g_top[r * G.top + i];
+            for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int j = 0; j < NV; ++j) v[j] += at == lane + L * j ? g : 0.f;
+                for (int i = 0; i < V; ++i) v[j][i] += c == (j < NV - 1 ? (lane + L * j) * V : last.at) + i ? g : 0.f;
         }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = lane + L * j;
-        if (c < G.classes) D[r * ldg + c] = static_cast<T>(v[j]);
-    }
+    for (int j = 0; j < NV; ++j)
+        if (j < NV - 1 || last.first < G.classes) store_from_f32<T, V>(out + (j < NV - 1 ? (lane + L * j) * V : last.at), v[j]);
 }
 
 // ---------------------------------------------------------------------------------------------
-// wide rows
+// wide rows: vector j of thread t covers the columns lo + (t + TH j) V ..
 // ---------------------------------------------------------------------------------------------
 // Partial results of a split row: Sums, then `top` keys.
-__device__ __forceinline__ int64_t partial_floats(int top) { return 4 + 2 * top; }
+__host__ __device__ constexpr int64_t partial_floats(int top) { return 4 + 2 * top; }
 
-// fn(value, column) for the columns lo, lo + 1, ... < hi of this thread, ascending; first(values) once per vector
-template <typename T, typename First, typename Fn>
-__device__ __forceinline__ void for_columns(const T* __restrict__ row, int lo, int hi, First first, Fn fn) {
-    constexpr int V = 16 / sizeof(T);
-    const int full = (hi - lo) / V;
-    for (int i = threadIdx.x; i < full; i += kWideThreads) {
-        float v[V];
-        load_as_f32<T, V>(row + lo + static_cast<int64_t>(i) * V, v);
-        first(v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) fn(v[j], lo + i * V + j);
-    }
-    const int c = lo + full * V + threadIdx.x;
-    if (c < hi) {
-        float v[1] = {static_cast<float>(row[c])};
-        first(v);
-        fn(v[0], c);
-    }
-}
-
+template <int TH>
 __device__ __forceinline__ key_t block_max_key(key_t k, key_t* lds) {
-#pragma unroll
-    for (int o = kWave / 2; o > 0; o >>= 1) {
-        const key_t other = shfl_xor_key(k, o);
-        k = other > k ? other : k;
-    }
+    k = lanes_max_key<kWave>(k);
     __syncthreads();
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = k;
     __syncthreads();
-    for (int w = 0; w < kWideThreads / kWave; ++w) k = lds[w] > k ? lds[w] : k;
-    return k;
+    return lanes_max_key<TH / kWave>(lds[threadIdx.x % (TH / kWave)]);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kWideThreads) void label_scores_wide(const T* __restrict__ Z, int64_t ld, int split_cols,
-                                                                  float* __restrict__ partial, Outputs O) {
+template <typename T, int TH, int NV>
+__global__ __launch_bounds__(TH) __attribute__((amdgpu_waves_per_eu(NV <= 4 ? 8 : 4))) void label_scores_wide(const T* __restrict__ Z, int64_t ld, int split_cols,
+                                                        float* __restrict__ partial, Outputs O) {
+    constexpr int V = 16 / sizeof(T);
     __shared__ key_t list[kList];
     __shared__ key_t found[kMaxTop];
-    __shared__ key_t wave_key[kWideThreads / kWave];
-    __shared__ Sums wave_sums[kWideThreads / kWave];
-    __shared__ key_t bound;
+    __shared__ key_t wave_key[TH / kWave];
+    __shared__ Sums wave_sums[TH / kWave];
+    __shared__ float part_max[kParts];
+    __shared__ float bound;
     __shared__ int listed;
     const int64_t r = blockIdx.x;
     const T* row = Z + r * ld;
     const int lo = blockIdx.y * split_cols, hi = min(O.classes, lo + split_cols);
-    Sums S{-kInf, 0.f, 0.f};
-    float base = 0.f;
-    unsigned best = 0, at = 0;
-    const bool top = O.top > 0;
-    for_columns<T>(
-        row, lo, hi,
-        [&](auto& v) {
-            float vm = S.m;
-            for (float x : v) vm = fmaxf(vm, x);
-            if (vm > S.m) {
-                S = join(S, Sums{vm, 0.f, 0.f});
-                base = vm;
-            }
-        },
-        [&](float x, int c) {
-            take(S, x, base);
-            if (top) {
-                const unsigned o = order_of(x);
-                if (o > best) { best = o; at = c; }
-            }
-        });
-    S = join_lanes<kWave>(S);
-    if (threadIdx.x % kWave == 0) wave_sums[threadIdx.x / kWave] = S;
+    auto place = [&](int j) { return place_of<V>(lo + (static_cast<int>(threadIdx.x) + TH * j) * V, hi); };
+    Raw<T, V> raw[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) raw[j] = load_raw<T, V>(row + place(j).at);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const Place p = place(j);
+        if (p.at < p.first) lowest(raw[j], p.first - p.at);
+    }
+    float my_max = -kInf;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) my_max = fmaxf(my_max, raw[j][i]);
+    forget(raw);                                           // unpacked again below: 8 values a vector are too many to keep
+    // part g: the columns of TH / kParts neighbouring threads; a NaN does not count for its part
+    const float part = lanes_max<TH / kParts>(my_max), wave_max = lanes_max<kWave>(my_max);
+    const int lane = threadIdx.x % kWave;
+    if (threadIdx.x % (TH / kParts) == 0) part_max[threadIdx.x / (TH / kParts)] = part;
+    if (lane == 0) wave_sums[threadIdx.x / kWave].m = wave_max;
     if (threadIdx.x < kMaxTop) found[threadIdx.x] = 0;
-    if (threadIdx.x == 0) { listed = 0; bound = 1; }
-    if (top) list[threadIdx.x] = best ? key_of(best, at) : 0;
+    if (threadIdx.x == 0) { listed = 0; bound = -kInf; }
     __syncthreads();
-    S = wave_sums[0];
-    for (int w = 1; w < kWideThreads / kWave; ++w) S = join(S, wave_sums[w]);
-    if (top) {
-        // part g: the columns of the threads g, g + kParts, ...
-        key_t part = 0;
-        if (threadIdx.x < kParts)
-            for (int i = threadIdx.x; i < kWideThreads; i += kParts) part = list[i] > part ? list[i] : part;
-        __syncthreads();
-        if (threadIdx.x < kParts) list[threadIdx.x] = part;
-        __syncthreads();
-        if (threadIdx.x < kParts) {
-            int above = 0;
-            for (int i = 0; i < kParts; ++i) above += list[i] > part ? 1 : 0;
-            if (above == O.top - 1 && part) bound = part;   // keys differ: one thread at most
+    Sums S{lanes_max<TH / kWave>(wave_sums[lane % (TH / kWave)].m), 0.f, 0.f};
+    const float base = S.m == -kInf ? 0.f : S.m;
+    if (O.entropy || gridDim.y > 1) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) take<true>(S, raw[j][i], base);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();
-        const key_t least = bound;
-        const unsigned least_order = static_cast<unsigned>(least >> 32);
-        for_columns<T>(row, lo, hi, [](auto&) {}, [&](float x, int c) {
-            const unsigned o = order_of(x);
-            if (o < least_order) return;
-            const key_t k = key_of(o, c);
-            if (k < least) return;
-            const int n = atomicAdd(&listed, 1);            // LDS; the ranks below do not depend on the order
-            if (n < kList) list[n] = k;
-        });
+        S.t = lanes_sum<kWave>(S.t);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) take<false>(S, raw[j][i], base);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    const bool odd = S.s != S.s;                           // a NaN or +inf among this thread's values
+    S.s = lanes_sum<kWave>(S.s);
+    forget(raw);
+    if (O.top > 0 && threadIdx.x < kParts) {
+        const float mine = part_max[threadIdx.x];
+        int above = 0, level = 0;
+#pragma unroll 8
+        for (int i = 0; i < kParts; ++i) {
+            above += part_max[i] > mine ? 1 : 0;
+            level += part_max[i] == mine ? 1 : 0;
+        }
+        if (above < O.top && above + level >= O.top) bound = mine;          // who writes, writes the same
+    }
+    if (lane == 0) { wave_sums[threadIdx.x / kWave].s = S.s; wave_sums[threadIdx.x / kWave].t = S.t; }
+    __syncthreads();
+    S.s = lanes_sum<TH / kWave>(wave_sums[lane % (TH / kWave)].s);
+    S.t = lanes_sum<TH / kWave>(wave_sums[lane % (TH / kWave)].t);
+    if (O.top > 0) {
+        const float least = bound;
+        if (!(my_max < least) || odd) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const Place p = place(j);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float x = raw[j][i];
+                    if (p.at + i < p.first || x < least) continue;
+                    const int n = atomicAdd(&listed, 1);    // LDS; the ranks below do not depend on the order
+                    if (n < kList) list[n] = key_of(order_of(x), p.at + i);
+                }
+            }
+        }
         __syncthreads();
         const int n = listed;
         if (n <= kList) {
-            for (int i = threadIdx.x; i < n; i += kWideThreads) {
+            for (int i = threadIdx.x; i < n; i += TH) {
                 const key_t k = list[i];
                 int above = 0;
                 for (int j = 0; j < n; ++j) above += list[j] > k ? 1 : 0;
                 if (above < O.top) found[above] = k;
             }
         } else {
-            key_t last = ~static_cast<key_t>(0);
-            for (int i = 0; i < O.top; ++i) {
-                key_t k = 0;
-                for_columns<T>(row, lo, hi, [](auto&) {}, [&](float x, int c) {
-                    const key_t q = key_of(order_of(x), c);
-                    if (q < last && q > k) k = q;
-                });
-                last = block_max_key(k, wave_key);
-                if (threadIdx.x == 0) found[i] = last;
+            key_t before = ~static_cast<key_t>(0);
+            for (int round = 0; round < O.top; ++round) {
+                const unsigned limit = static_cast<unsigned>(before >> 32), limit_at = index_of(before);
+                unsigned best = 0, at = 0;
+                forget(raw);                               // orders of all values would not fit the registers
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    const Place p = place(j);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const unsigned o = order_of(raw[j][i]), c = p.at + i;
+                        // after the last one found, and better than this thread's best (whose column is lower)
+                        if (p.at + i >= p.first && (o < limit || (o == limit && c > limit_at)) && o > best) { best = o; at = c; }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                const key_t k = best ? key_of(best, at) : 0;
+                before = block_max_key<TH>(k, wave_key);
+                if (threadIdx.x == 0) found[round] = before;
             }
         }
         __syncthreads();
@@ -381,25 +439,24 @@ constexpr int kMaxSplits = 64;
 
 // Joins the splits of a row: one workgroup per row.
 template <typename T>
-__global__ __launch_bounds__(256) void label_scores_join(const T* __restrict__ Z, int64_t ld, int splits, const float* __restrict__ partial,
-                                                         Outputs O) {
+__global__ __launch_bounds__(kThreads) void label_scores_join(const T* __restrict__ Z, int64_t ld, int splits,
+                                                              const float* __restrict__ partial, Outputs O) {
     __shared__ key_t list[kMaxSplits * kMaxTop];
     const int64_t r = blockIdx.x;
     const float* in = partial + r * splits * partial_floats(O.top);
-    const int lane = threadIdx.x % kWave;
+    const int lane = threadIdx.x % kWave, n = splits * O.top;
+    for (int i = threadIdx.x; i < n; i += kThreads)
+        list[i] = reinterpret_cast<const key_t*>(in + (i / O.top) * partial_floats(O.top) + 4)[i % O.top];
     Sums S{-kInf, 0.f, 0.f};
     if (lane < splits) {
         const float* p = in + lane * partial_floats(O.top);
         S = Sums{p[0], p[1], p[2]};
     }
-    S = join_lanes<kWave>(S);
+    S = lanes_join<kWave>(S);
     const Final F = finish(S);
     if (threadIdx.x == 0) write_scores<T>(O, Z + r * ld, r, F);
-    const int n = splits * O.top;
-    for (int i = threadIdx.x; i < n; i += 256)
-        list[i] = reinterpret_cast<const key_t*>(in + (i / O.top) * partial_floats(O.top) + 4)[i % O.top];
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 256) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
         const key_t k = list[i];
         if (!k) continue;                                   // a split with fewer columns than `top`
         int above = 0;
@@ -408,72 +465,119 @@ __global__ __launch_bounds__(256) void label_scores_join(const T* __restrict__ Z
     }
 }
 
+constexpr int kGradVectors = 8;            // most vectors of a thread in the wide backward
+
 template <typename T>
-__global__ __launch_bounds__(kWideThreads) void label_grads_wide(const T* __restrict__ Z, T* __restrict__ D, int64_t ld, int64_t ldg,
-                                                                 int split_cols, Grads G) {
+__global__ __launch_bounds__(kThreads) void label_grads_wide(const T* __restrict__ Z, T* __restrict__ D, int64_t ld, int64_t ldg,
+                                                             int split_cols, Grads G) {
     constexpr int V = 16 / sizeof(T);
     const int64_t r = blockIdx.x;
     const T* row = Z + r * ld;
     T* out = D + r * ldg;
     const int lo = blockIdx.y * split_cols, hi = min(G.classes, lo + split_cols);
     const RowGrad R = row_grad(G, r);
+    const bool h = G.g_entropy != nullptr;
     const int full = (hi - lo) / V;
-    for (int i = threadIdx.x; i < full; i += kWideThreads) {
+#pragma unroll 2
+    for (int i = threadIdx.x; i < full; i += kThreads) {
         const int c = lo + i * V;
+        const Raw<T, V> raw = load_raw<T, V>(row + c);
         float v[V];
-        load_as_f32<T, V>(row + c, v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = grad_of(R, v[j], c + j);
+        for (int j = 0; j < V; ++j) v[j] = h ? grad_of<true>(R, raw[j], c + j) : grad_of<false>(R, raw[j], c + j);
         store_from_f32<T, V>(out + c, v);
     }
     const int c = lo + full * V + threadIdx.x;
-    if (c < hi) out[c] = static_cast<T>(grad_of(R, static_cast<float>(row[c]), c));
+    if (c < hi) out[c] = static_cast<T>(grad_of<true>(R, static_cast<float>(row[c]), c));
     if (!G.g_top || !R.any) return;                         // the same for the whole workgroup
     __syncthreads();                                        // the stores above are over: these few go on top of them
     if (static_cast<int>(threadIdx.x) < G.top) {
         const int64_t at = G.top_index[r * G.top + threadIdx.x];
         if (at >= lo && at < hi)
-            out[at] = static_cast<T>(grad_of(R, static_cast<float>(row[at]), static_cast<int>(at)) + G.g_top[r * G.top + threadIdx.x]);
+            out[at] = static_cast<T>(grad_of<true>(R, static_cast<float>(row[at]), static_cast<int>(at)) + G.g_top[r * G.top + threadIdx.x]);
     }
 }
 
-// Splits of a wide row's columns: enough workgroups for two per CU, at least 4096 columns each.
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+constexpr int kNarrowClasses = 1024;
+constexpr int kWideThreads = 1024, kWideVectors = 8;
+
+// Splits of a wide row's columns: as many as its length needs (a workgroup's registers hold kWideThreads kWideVectors
+// vectors), more where rows are few, for two workgroups per CU of at least 4096 columns each.
 struct Splits { int n, cols; };
-Splits splits_of(int rows, int classes) {
-    const int want = std::min({kMaxSplits, std::max(1, 512 / std::max(rows, 1)), std::max(1, classes / 4096)});
-    const int cols = ((classes + want - 1) / want + 7) / 8 * 8;
+Splits splits_of(int rows, int classes, int dtype) {
+    const int V = 16 / element_bytes(dtype), most = kWideThreads * kWideVectors * V;
+    const int need = (classes + most - 1) / most;
+    const int want = std::max(need, std::min({kMaxSplits, std::max(1, 512 / std::max(rows, 1)), std::max(1, classes / 4096)}));
+    const int cols = ((classes + want - 1) / want + V - 1) / V * V;
     return {(classes + cols - 1) / cols, cols};
 }
-
-constexpr int kNarrowClasses = 1024;
+constexpr int kMaxClasses = CBM_LABELS_MAX_CLASSES;
+static_assert(kMaxClasses == kMaxSplits * kWideThreads * kWideVectors * 4, "fp32: the fewest columns a split holds");
 
 #define CBM_LABEL_BY_TYPE(CALL)                          \
     if (dtype == CBM_DTYPE_F32) { CALL(float) }          \
     else if (dtype == CBM_DTYPE_BF16) { CALL(__bf16) }   \
     else { CALL(_Float16) }
-// Lanes of a row: the fewest that leave each at most 8 values (16 in a whole wavefront).
-#define CBM_LABEL_BY_WIDTH(T, CALL)                      \
-    if (classes <= 32) { CALL(T, 4, 8) }                 \
-    else if (classes <= 64) { CALL(T, 8, 8) }            \
-    else if (classes <= 128) { CALL(T, 16, 8) }          \
-    else if (classes <= 256) { CALL(T, 32, 8) }          \
-    else if (classes <= 512) { CALL(T, 64, 8) }          \
-    else { CALL(T, 64, 16) }
+// Lanes of a row and vectors of a lane: the fewest lanes that hold the row in at most 16 (two-byte types: 24) values each.
+#define CBM_LABEL_BY_WIDTH(T, CALL)                                                     \
+    if constexpr (sizeof(T) == 4) {                                                     \
+        if (classes < 4) { CALL(T, 1, 4, 1) }                                           \
+        else if (classes <= 16) { CALL(T, 4, 4, 1) }                                    \
+        else if (classes <= 32) { CALL(T, 4, 4, 2) }                                    \
+        else if (classes <= 48) { CALL(T, 4, 4, 3) }                                    \
+        else if (classes <= 64) { CALL(T, 4, 4, 4) }                                    \
+        else if (classes <= 96) { CALL(T, 4, 8, 3) }                                    \
+        else if (classes <= 128) { CALL(T, 4, 8, 4) }                                   \
+        else if (classes <= 192) { CALL(T, 4, 16, 3) }                                  \
+        else if (classes <= 256) { CALL(T, 4, 16, 4) }                                  \
+        else if (classes <= 384) { CALL(T, 4, 32, 3) }                                  \
+        else if (classes <= 512) { CALL(T, 4, 32, 4) }                                  \
+        else if (classes <= 768) { CALL(T, 4, 64, 3) }                                  \
+        else { CALL(T, 4, 64, 4) }                                                      \
+    } else {                                                                            \
+        if (classes < 8) { CALL(T, 1, 8, 1) }                                           \
+        else if (classes <= 32) { CALL(T, 8, 4, 1) }                                    \
+        else if (classes <= 64) { CALL(T, 8, 4, 2) }                                    \
+        else if (classes <= 96) { CALL(T, 8, 4, 3) }                                    \
+        else if (classes <= 128) { CALL(T, 8, 8, 2) }                                   \
+        else if (classes <= 192) { CALL(T, 8, 8, 3) }                                   \
+        else if (classes <= 256) { CALL(T, 8, 16, 2) }                                  \
+        else if (classes <= 384) { CALL(T, 8, 16, 3) }                                  \
+        else if (classes <= 512) { CALL(T, 8, 32, 2) }                                  \
+        else if (classes <= 768) { CALL(T, 8, 32, 3) }                                  \
+        else { CALL(T, 8, 64, 2) }                                                      \
+    }
+// Threads of a wide row and vectors of a thread: 256 threads up to 32 KiB, 1024 up to 128 KiB.
+#define CBM_LABEL_BY_SPLIT(T, CALL)                                                     \
+    {                                                                                   \
+        const int vectors = (s.cols * static_cast<int>(sizeof(T)) + 15) / 16;           \
+        if (vectors <= 256) { CALL(T, 256, 1) }                                         \
+        else if (vectors <= 512) { CALL(T, 256, 2) }                                    \
+        else if (vectors <= 1024) { CALL(T, 256, 4) }                                   \
+        else if (vectors <= 2048) { CALL(T, 256, 8) }                                   \
+        else if (vectors <= 4096) { CALL(T, 1024, 4) }                                  \
+        else { CALL(T, 1024, 8) }                                                       \
+    }
 
 int check_labels(int rows, int classes, int top, int64_t ld, int dtype) {
     if (dtype < CBM_DTYPE_F32 || dtype > CBM_DTYPE_F16) return CBM_ERR_SHAPE;
-    if (rows < 0 || classes < 1 || classes > (1 << 30) || top < 0 || top > kMaxTop || top > classes || ld < classes) return CBM_ERR_SHAPE;
+    if (rows < 0 || classes < 1 || classes > kMaxClasses || top < 0 || top > kMaxTop || top > classes || ld < classes) return CBM_ERR_SHAPE;
     return CBM_OK;
 }
+
+unsigned narrow_blocks(int rows, int L) { return static_cast<unsigned>((static_cast<int64_t>(rows) * L + kThreads - 1) / kThreads); }
 
 }  // namespace
 
 extern "C" {
 
-int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t top) {
-    if (rows <= 0 || classes <= kNarrowClasses || top < 0 || top > kMaxTop) return 0;
-    const Splits s = splits_of(rows, classes);
-    return s.n > 1 ? static_cast<int64_t>(rows) * s.n * (4 + 2 * top) : 0;
+int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t top, int32_t dtype) {
+    if (check_labels(rows, classes, top, classes, dtype) || rows == 0 || classes <= kNarrowClasses) return 0;
+    const Splits s = splits_of(rows, classes, dtype);
+    return s.n > 1 ? static_cast<int64_t>(rows) * s.n * partial_floats(top) : 0;
 }
 
 int cbm_label_scores(const void* logits, const int64_t* labels, float* logp, float* entropy, float* top_logp, int64_t* top_index,
@@ -485,26 +589,32 @@ int cbm_label_scores(const void* logits, const int64_t* labels, float* logp, flo
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Outputs O{labels, logp, entropy, top_logp, top_index, stats, ignore_index, classes, top};
     if (classes <= kNarrowClasses) {
-#define NARROW(T, L, NV)                                                                                                      \
-    hipLaunchKernelGGL((label_scores_narrow<T, L, NV>), dim3((unsigned)((static_cast<int64_t>(rows) * L + kNarrowThreads - 1) / kNarrowThreads)), \
-                       dim3(kNarrowThreads), 0, st, static_cast<const T*>(logits), ld, rows, O);
+#define NARROW(T, V, L, NV)                                                                                                  \
+    if (entropy || top > 0)                                                                                                  \
+        hipLaunchKernelGGL((label_scores_narrow<T, V, L, NV, true>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,    \
+                           static_cast<const T*>(logits), ld, rows, O);                                                      \
+    else                                                                                                                     \
+        hipLaunchKernelGGL((label_scores_narrow<T, V, L, NV, false>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,   \
+                           static_cast<const T*>(logits), ld, rows, O);
 #define BY_WIDTH(T) CBM_LABEL_BY_WIDTH(T, NARROW)
         CBM_LABEL_BY_TYPE(BY_WIDTH)
 #undef BY_WIDTH
 #undef NARROW
         return check_launch();
     }
-    const Splits s = splits_of(rows, classes);
+    const Splits s = splits_of(rows, classes, dtype);
     if (s.n > 1 && !workspace) return CBM_ERR_NULL;
-#define WIDE(T)                                                                                                             \
-    hipLaunchKernelGGL(label_scores_wide<T>, dim3(rows, s.n), dim3(kWideThreads), 0, st, static_cast<const T*>(logits), ld, \
+#define WIDE(T, TH, NV)                                                                                                     \
+    hipLaunchKernelGGL((label_scores_wide<T, TH, NV>), dim3(rows, s.n), dim3(TH), 0, st, static_cast<const T*>(logits), ld, \
                        s.cols, workspace, O);
+#define BY_SPLIT(T) CBM_LABEL_BY_SPLIT(T, WIDE)
 #define JOIN(T) \
-    hipLaunchKernelGGL(label_scores_join<T>, dim3(rows), dim3(256), 0, st, static_cast<const T*>(logits), ld, s.n, workspace, O);
-    CBM_LABEL_BY_TYPE(WIDE)
+    hipLaunchKernelGGL(label_scores_join<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(logits), ld, s.n, workspace, O);
+    CBM_LABEL_BY_TYPE(BY_SPLIT)
     if (int rc = check_launch()) return rc;
     if (s.n > 1) { CBM_LABEL_BY_TYPE(JOIN) }
 #undef WIDE
+#undef BY_SPLIT
 #undef JOIN
     return check_launch();
 }
@@ -520,19 +630,22 @@ int cbm_label_scores_backward(const void* logits, const int64_t* labels, const f
     hipStream_t st = static_cast<hipStream_t>(stream);
     const Grads G{labels, stats, entropy, top_index, g_logp, g_entropy, g_top, ignore_index, classes, top};
     if (classes <= kNarrowClasses) {
-#define NARROW(T, L, NV)                                                                                                     \
-    hipLaunchKernelGGL((label_grads_narrow<T, L, NV>), dim3((unsigned)((static_cast<int64_t>(rows) * L + kNarrowThreads - 1) / kNarrowThreads)), \
-                       dim3(kNarrowThreads), 0, st, static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, rows, G);
+#define NARROW(T, V, L, NV)                                                                                             \
+    hipLaunchKernelGGL((label_grads_narrow<T, V, L, NV>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,          \
+                       static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, rows, G);
 #define BY_WIDTH(T) CBM_LABEL_BY_WIDTH(T, NARROW)
         CBM_LABEL_BY_TYPE(BY_WIDTH)
 #undef BY_WIDTH
 #undef NARROW
         return check_launch();
     }
-    const Splits s = splits_of(rows, classes);
-#define WIDE(T)                                                                                                            \
-    hipLaunchKernelGGL(label_grads_wide<T>, dim3(rows, s.n), dim3(kWideThreads), 0, st, static_cast<const T*>(logits),     \
-                       static_cast<T*>(grad), ld, ldg, s.cols, G);
+    // a workgroup per share of a row: kGradVectors vectors a thread, fewer where rows are few
+    const int V = 16 / element_bytes(dtype);
+    int cols = kThreads * kGradVectors * V;
+    while (cols > kThreads * V && static_cast<int64_t>(rows) * ((classes + cols - 1) / cols) < 1024) cols >>= 1;
+#define WIDE(T)                                                                                                               \
+    hipLaunchKernelGGL(label_grads_wide<T>, dim3(rows, (classes + cols - 1) / cols), dim3(kThreads), 0, st,                   \
+                       static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, cols, G);
     CBM_LABEL_BY_TYPE(WIDE)
 #undef WIDE
     return check_launch();

@@ -41,7 +41,7 @@ def _forward(z, labels, entropy, top, ignore_index, keep):
     top_logp = torch.empty((rows, top), **f32) if top else None
     top_index = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
     stats = torch.empty((rows, 2), **f32) if keep else None
-    floats = lib.cbm_label_scores_workspace_floats(rows, classes, top)
+    floats = lib.cbm_label_scores_workspace_floats(rows, classes, top, DTYPES[z.dtype])
     ws = torch.empty(floats, **f32) if floats else None
     with on_device(dev):
         rc = lib.cbm_label_scores(ptr(z), ptr(labels), ptr(logp), ptr(ent), ptr(top_logp), ptr(top_index), ptr(stats), ptr(ws), rows,
@@ -96,8 +96,8 @@ def label_log_probs(logits, labels=None, *, entropy=False, top=0, ignore_index=-
     if not 0 <= top <= min(_lib.CBM_LABELS_MAX_TOP, classes):
         raise ValueError(f"top must be between 0 and {min(_lib.CBM_LABELS_MAX_TOP, classes)}, got {top}")
     check_int32(rows, "rows of logits")
-    if classes > 1 << 30:
-        raise ValueError(f"{classes} classes: at most {1 << 30}")
+    if classes > _lib.CBM_LABELS_MAX_CLASSES:
+        raise ValueError(f"{classes} classes: at most {_lib.CBM_LABELS_MAX_CLASSES}")
     lead = logits.shape[:-1]
     if labels is not None:
         if not isinstance(labels, torch.Tensor):

@@ -656,8 +656,8 @@ int cbm_group_norm_backward(const cbm_norm_batch* batch, const void* X_dev, cons
  *   stats   [rows, 2] fp32 (nullable)    what the backward needs: {max, log sum exp(logit - max)}
  * A row of -inf alone has log probabilities -inf and entropy 0; a NaN or +inf in a row makes its scores NaN.
  * workspace: cbm_label_scores_workspace_floats() floats, may be NULL if that is 0. */
-enum { CBM_LABELS_MAX_TOP = 32 };
-int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t top);
+enum { CBM_LABELS_MAX_TOP = 32, CBM_LABELS_MAX_CLASSES = 64 * 1024 * 8 * 4 };   /* 2 Mi classes */
+int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t top, int32_t dtype);
 int cbm_label_scores(const void* logits_dev, const int64_t* labels_dev, float* logp_dev, float* entropy_dev, float* top_logp_dev,
                      int64_t* top_index_dev, float* stats_dev, float* workspace_dev, int32_t rows, int32_t classes, int32_t top,
                      int64_t ld, int64_t ignore_index, int32_t dtype, void* stream);

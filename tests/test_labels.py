@@ -163,6 +163,13 @@ def test_rows_that_crowd_the_likeliest_classes(gpu):
     zb = torch.rand((rows, classes), generator=g)
     zb[0] += 5.0 * (part < 31)
     check(gpu, zb.to(BF16), y, 32, "crowded bf16")
+    zc = torch.rand((rows, classes), generator=g)
+    zc[0, 4096:9000] += 5.0                                # neighbouring columns
+    zc[1, :3000:2] += 5.0
+    zc[2] = 0.0
+    zc[3, 10000:10040] += 5.0
+    check(gpu, zc, y, 32, "crowded neighbours")
+    check(gpu, zc.to(BF16), y, 32, "crowded neighbours bf16")
 
 
 @pytest.mark.gpu
