@@ -18,10 +18,16 @@
 //     apply  X [s, l] = a X + B X    rows of B against rows of X^T;  writes X, X^T, or the result
 // Sides are padded to whole tiles with zeros, which all three products keep: the inner loops check no bounds.
 // A list of matrices shares its launches: the tiles of all of them are one grid.
+//
+// Three shapes of the same product, chosen launch by launch by how many tiles there are (see choose()):
+//     tiles of 128 or 64   operands through LDS, copied there directly (no registers in between) one stage ahead;
+//     tiles of 32          for small matrices, where a product is one latency after another: eight wavefronts share a tile
+//                          and split k, operands straight to registers, partial sums joined in LDS.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "dense_types.h"
@@ -30,11 +36,12 @@ namespace {
 
 using namespace cbm_dense;
 
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kMaxItems = CBM_ORTHO_MAX_ITEMS;
-constexpr int kNormBlocks = 64;            // partial sums of squares per matrix
+constexpr int kNormBlocks = 256;           // partial sums of squares per matrix, at most
 constexpr float kLo = 2048.f;
 
 struct Item {
@@ -43,39 +50,61 @@ struct Item {
     float* weight;
     float* momentum;
     int64_t ld_src, ld_dst, ld_weight, ld_momentum;
-    int rows, cols, sp, lp;                // sp, lp: short and long side, padded
+    int rows, cols, sp, lp;                // sp, lp: short and long side, padded to tiles
+    int ls, ll;                            // halves from row to row of planes whose rows run along the short / long side
+    int norm_blocks;
     int64_t base;                          // first half of the item's planes in the workspace
 };
 
+// The list a turn works on.  A kernel's arguments lie in host memory, and every workgroup would fetch its item from there:
+// the first launch writes the list into the workspace, the others read it there.
+enum Grid { kSplitGrid, kSquareGrid, kWideGrid, kGrids };
 struct Items {
     Item it[kMaxItems];
+    int ends[kGrids][kMaxItems];           // tiles up to and with each item, in each of the grids
     int n;
 };
+
+// The item that workgroup b of a grid works on; b becomes its place in the item.  One load, whatever the number of items
+// (walking along the list, a load after another, cost 1 us per item).
+__device__ __forceinline__ int item_of(const Items& L, Grid grid, int& b) {
+    const int end = L.ends[grid][min(static_cast<int>(threadIdx.x) % kWave, kMaxItems - 1)];
+    const int k = min(__popcll(__ballot(end <= b)), kMaxItems - 1);
+    if (k > 0) b -= __builtin_amdgcn_readlane(end, k - 1);
+    return k;
+}
 
 struct Update {
     float lr, mu, decay;
     int nesterov, on;
 };
 
-// Planes of an item, in halves from its base: X hi lo [sp, lp], X^T hi lo [lp, sp] twice (read and written in turns),
-// A hi lo and B hi lo [sp, sp].
-struct Planes { _Float16 *x, *xt[2], *a, *b; int64_t nx, na; };
+// Planes of an item, in halves from its base: X hi lo [sp, ll], X^T hi lo [lp, ls] twice (read and written in turns),
+// A hi lo and B hi lo [sp, ls].
+struct Planes { _Float16 *x, *xt[2], *a, *b; int64_t nx, nt, na; };   // n: from the hi to the lo plane
 __device__ __forceinline__ Planes planes_of(const Item& I, _Float16* ws) {
     Planes P;
-    P.nx = static_cast<int64_t>(I.sp) * I.lp;
-    P.na = static_cast<int64_t>(I.sp) * I.sp;
+    P.nx = static_cast<int64_t>(I.sp) * I.ll;
+    P.nt = static_cast<int64_t>(I.lp) * I.ls;
+    P.na = static_cast<int64_t>(I.sp) * I.ls;
     P.x = ws + I.base;
     P.xt[0] = P.x + 2 * P.nx;
-    P.xt[1] = P.xt[0] + 2 * P.nx;
-    P.a = P.xt[1] + 2 * P.nx;
+    P.xt[1] = P.xt[0] + 2 * P.nt;
+    P.a = P.xt[1] + 2 * P.nt;
     P.b = P.a + 2 * P.na;
     return P;
 }
-int64_t item_halves(int sp, int lp) { return 6LL * sp * lp + 4LL * sp * sp; }
+int64_t item_halves(const Item& I) { return 2LL * I.sp * I.ll + 4LL * I.lp * I.ls + 4LL * I.sp * I.ls; }
 
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
     hi = static_cast<_Float16>(v);
     lo = static_cast<_Float16>((v - static_cast<float>(hi)) * kLo);
+}
+__device__ __forceinline__ void split4(float v, half4& hi, half4& lo, int e) {
+    _Float16 a, b;
+    split(v, a, b);
+    hi[e] = a;
+    lo[e] = b;
 }
 __device__ __forceinline__ float whole(_Float16 hi, _Float16 lo) {
     return __builtin_fmaf(static_cast<float>(lo), 1.f / kLo, static_cast<float>(hi));
@@ -84,74 +113,113 @@ __device__ __forceinline__ float whole(_Float16 hi, _Float16 lo) {
 // ---------------------------------------------------------------------------------------------
 // |G|_F, the momentum, and the planes of X
 // ---------------------------------------------------------------------------------------------
+// Workgroup (block of rows, item): sums of squares in 64 bits (a matrix of 1e20s has no norm in 32).  Wavefront w takes
+// the rows w of every four, kFetch strides of 64 columns in flight: places outside read the matrix's last element and
+// count as nothing, for a branch around each load made the loads wait for one another.
+constexpr int kFetch = 8;
 template <typename T>
-__device__ __forceinline__ float source(const Item& I, const Update& U, int r, int c) {
-    const float g = static_cast<float>(static_cast<const T*>(I.src)[static_cast<int64_t>(r) * I.ld_src + c]);
-    if (!U.on) return g;
-    const float m = I.momentum[static_cast<int64_t>(r) * I.ld_momentum + c];
-    return U.nesterov ? __builtin_fmaf(U.mu, m, g) : m;
-}
-
-// Workgroup (block of rows, item): sums of squares in 64 bits (a matrix of 1e20s has no norm in 32).
-template <typename T>
-__global__ __launch_bounds__(256) void ortho_norms(Items L, Update U, double* __restrict__ partial) {
-    __shared__ double red[256];
-    const Item& I = L.it[blockIdx.y];
+__global__ __launch_bounds__(256) void ortho_norms(Items L, Update U, Items* __restrict__ list, double* __restrict__ partial) {
+    __shared__ double red[4];
+    const Item I = L.it[blockIdx.y];
+    if (blockIdx.x == 0 && threadIdx.x == 0) list->it[blockIdx.y] = I;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < kGrids * kMaxItems)
+        list->ends[threadIdx.x / kMaxItems][threadIdx.x % kMaxItems] = L.ends[threadIdx.x / kMaxItems][threadIdx.x % kMaxItems];
+    if (static_cast<int>(blockIdx.x) >= I.norm_blocks) return;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     double sum = 0.0;
-    for (int r = blockIdx.x; r < I.rows; r += kNormBlocks)
-        for (int c = threadIdx.x; c < I.cols; c += 256) {
+    for (int r = blockIdx.x * 4 + wave; r < I.rows; r += I.norm_blocks * 4) {
+        const T* row = static_cast<const T*>(I.src) + static_cast<int64_t>(r) * I.ld_src;
+        float* momentum = I.momentum + static_cast<int64_t>(r) * I.ld_momentum;
+        for (int c0 = lane; c0 < I.cols; c0 += kWave * kFetch) {
+            T g[kFetch];
+            float v[kFetch];
+#pragma unroll
+            for (int f = 0; f < kFetch; ++f) g[f] = row[min(c0 + f * kWave, I.cols - 1)];
             if (U.on) {
-                float* m = I.momentum + static_cast<int64_t>(r) * I.ld_momentum + c;
-                const float g = static_cast<float>(static_cast<const T*>(I.src)[static_cast<int64_t>(r) * I.ld_src + c]);
-                *m = __builtin_fmaf(U.mu, *m, g);
+#pragma unroll
+                for (int f = 0; f < kFetch; ++f) v[f] = momentum[min(c0 + f * kWave, I.cols - 1)];
+#pragma unroll
+                for (int f = 0; f < kFetch; ++f) {
+                    v[f] = __builtin_fmaf(U.mu, v[f], static_cast<float>(g[f]));
+                    if (c0 + f * kWave < I.cols) momentum[c0 + f * kWave] = v[f];
+                    if (U.nesterov) v[f] = __builtin_fmaf(U.mu, v[f], static_cast<float>(g[f]));
+                }
+            } else {
+#pragma unroll
+                for (int f = 0; f < kFetch; ++f) v[f] = static_cast<float>(g[f]);
             }
-            const double v = source<T>(I, U, r, c);
-            sum += v * v;
+#pragma unroll
+            for (int f = 0; f < kFetch; ++f)
+                sum += c0 + f * kWave < I.cols ? static_cast<double>(v[f]) * v[f] : 0.0;
         }
-    red[threadIdx.x] = sum;
-    __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-        if (static_cast<int>(threadIdx.x) < h) red[threadIdx.x] += red[threadIdx.x + h];
-        __syncthreads();
     }
-    if (threadIdx.x == 0) partial[blockIdx.y * kNormBlocks + blockIdx.x] = red[0];
+#pragma unroll
+    for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[blockIdx.y * kNormBlocks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // Tile of 64 x 64 of X in the orientation short x long: both orders of the planes, zeros in the padding.
 template <typename T>
-__global__ __launch_bounds__(256) void ortho_split(Items L, Update U, const double* __restrict__ partial, float eps, _Float16* __restrict__ ws) {
+__global__ __launch_bounds__(256) void ortho_split(const Items* __restrict__ list, Update U, const double* __restrict__ partial, float eps, _Float16* __restrict__ ws) {
     __shared__ float tile[64][65];
-    int b = blockIdx.x, k = 0;
-    for (;; ++k) {                                          // the grid is the sum of the items' tiles
-        const int t = (L.it[k].sp / 64) * (L.it[k].lp / 64);
-        if (b < t) break;
-        b -= t;
-    }
-    const Item& I = L.it[k];
+    __shared__ double red[4];
+    const Items& L = *list;
+    int b = blockIdx.x;
+    const int k = item_of(L, kSplitGrid, b);
+    const Item I = L.it[k];
     const Planes P = planes_of(I, ws);
-    const int i0 = b / (I.lp / 64) * 64, j0 = b % (I.lp / 64) * 64;
-    double sum = 0.0;
-    for (int i = 0; i < kNormBlocks; ++i) sum += partial[k * kNormBlocks + i];
-    const float inv = static_cast<float>(1.0 / (sqrt(sum) + static_cast<double>(eps)));
+    const int across = (I.lp + 63) / 64, i0 = b / across * 64, j0 = b % across * 64;
+    double sum = static_cast<int>(threadIdx.x) < I.norm_blocks ? partial[k * kNormBlocks + threadIdx.x] : 0.0;
     const bool tall = I.rows > I.cols;
     const int tx = threadIdx.x % 64, ty = threadIdx.x / 64;
-    for (int y = ty; y < 64; y += 4) {
-        // memory order: rows of G run along tx
-        const int r = (tall ? j0 : i0) + y, c = (tall ? i0 : j0) + tx;
-        const float v = r < I.rows && c < I.cols ? source<T>(I, U, r, c) * inv : 0.f;
-        tile[tall ? tx : y][tall ? y : tx] = v;             // [short][long]
+    // Rows of G run along tx.  As above, the padding reads the matrix's edge, and is set to zero afterwards.
+    const int r0 = (tall ? j0 : i0) + ty, c = (tall ? i0 : j0) + tx, cc = min(c, I.cols - 1);
+    T g[16];
+    float v[16];
+#pragma unroll
+    for (int y = 0; y < 16; ++y) g[y] = static_cast<const T*>(I.src)[static_cast<int64_t>(min(r0 + 4 * y, I.rows - 1)) * I.ld_src + cc];
+    if (U.on) {                                             // the momentum is up to date already
+#pragma unroll
+        for (int y = 0; y < 16; ++y) v[y] = I.momentum[static_cast<int64_t>(min(r0 + 4 * y, I.rows - 1)) * I.ld_momentum + cc];
+#pragma unroll
+        for (int y = 0; y < 16; ++y)
+            if (U.nesterov) v[y] = __builtin_fmaf(U.mu, v[y], static_cast<float>(g[y]));
+    } else {
+#pragma unroll
+        for (int y = 0; y < 16; ++y) v[y] = static_cast<float>(g[y]);
     }
+#pragma unroll
+    for (int y = 0; y < 16; ++y)
+        if (c >= I.cols || r0 + 4 * y >= I.rows) v[y] = 0.f;
+#pragma unroll
+    for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = sum;
     __syncthreads();
-    for (int y = ty; y < 64; y += 4) {
-        _Float16 hi, lo;
-        split(tile[y][tx], hi, lo);
-        const int64_t at = static_cast<int64_t>(i0 + y) * I.lp + j0 + tx;
-        P.x[at] = hi;
-        P.x[P.nx + at] = lo;
-        split(tile[tx][y], hi, lo);
-        const int64_t to = static_cast<int64_t>(j0 + y) * I.sp + i0 + tx;
-        P.xt[0][to] = hi;
-        P.xt[0][P.nx + to] = lo;
+    const float inv = static_cast<float>(1.0 / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + static_cast<double>(eps)));
+#pragma unroll
+    for (int y = 0; y < 16; ++y) tile[tall ? tx : ty + 4 * y][tall ? ty + 4 * y : tx] = v[y] * inv;     // [short][long]
+    __syncthreads();
+    const int f = threadIdx.x % 16 * 4;                     // sides are multiples of 32: four halves are inside or outside
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+        const int u = threadIdx.x / 16 + 16 * y;
+        half4 hi, lo;
+        if (i0 + u < I.sp && j0 + f < I.lp) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split4(tile[u][f + e], hi, lo, e);
+            const int64_t at = static_cast<int64_t>(i0 + u) * I.ll + j0 + f;
+            *reinterpret_cast<half4*>(P.x + at) = hi;
+            *reinterpret_cast<half4*>(P.x + P.nx + at) = lo;
+        }
+        if (j0 + u < I.lp && i0 + f < I.sp) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split4(tile[f + e][u], hi, lo, e);
+            const int64_t to = static_cast<int64_t>(j0 + u) * I.ls + i0 + f;
+            *reinterpret_cast<half4*>(P.xt[0] + to) = hi;
+            *reinterpret_cast<half4*>(P.xt[0] + P.nt + to) = lo;
+        }
     }
 }
 
@@ -162,167 +230,411 @@ enum Kind { kGram, kPoly, kApply, kResult };
 
 struct Poly { float a, b, c; };
 
+constexpr bool symmetric(Kind k) { return k == kGram || k == kPoly; }
+
+// Which tile of which item a workgroup computes.
+struct Tile { int item, i0, j0; };
+
+// Workgroups are dealt to the 8 XCDs in turn; each gets a contiguous range of the tiles, which run down groups of four
+// tile rows, so that an XCD's tiles share their operands in its L2.
+template <Kind KIND, int TILE>
+__device__ __forceinline__ Tile tile_of(const Items& L) {
+    constexpr int kXcds = 8, kGroup = 4;
+    const int nb = gridDim.x, x = blockIdx.x % kXcds, q = nb / kXcds, rest = nb % kXcds;
+    int b = x * q + min(x, rest) + blockIdx.x / kXcds;
+    const int k = item_of(L, symmetric(KIND) ? kSquareGrid : kWideGrid, b);
+    if constexpr (symmetric(KIND)) {
+        int bj = static_cast<int>((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
+        while (bj * (bj + 1) / 2 > b) --bj;
+        while ((bj + 1) * (bj + 2) / 2 <= b) ++bj;
+        return {k, (b - bj * (bj + 1) / 2) * TILE, bj * TILE};      // i0 <= j0
+    } else {
+        const int mt = L.it[k].sp / TILE, nt = L.it[k].lp / TILE;
+        const int g = b / (kGroup * nt), r = b - g * kGroup * nt, rows = min(kGroup, mt - g * kGroup);
+        return {k, (g * kGroup + r % rows) * TILE, r / rows * TILE};
+    }
+}
+
+// The operands of a tile: P rows from i0, Q rows from j0, along k; the lo plane lies pn (qn) halves after the hi plane.
+struct Operands { const _Float16 *p, *q; int64_t pn, qn; int K, ld; };
+template <Kind KIND>
+__device__ __forceinline__ Operands operands_of(const Item& I, const Planes& P, const Tile& t, int turn) {
+    Operands O;
+    if constexpr (KIND == kGram) O = {P.x, P.x, P.nx, P.nx, I.lp, I.ll};
+    else if constexpr (KIND == kPoly) O = {P.a, P.a, P.na, P.na, I.sp, I.ls};
+    else O = {P.b, P.xt[turn], P.na, P.nt, I.sp, I.ls};
+    O.p += static_cast<int64_t>(t.i0) * O.ld;
+    O.q += static_cast<int64_t>(t.j0) * O.ld;
+    return O;
+}
+
+// What a product leaves for four rows i .. i + 3 of column j, given their sums in v: the new values, which go to X^T, A or
+// B (four halves along memory) and come back as words {hi, lo} for the row order, or as they are for the result.
+template <Kind KIND>
+__device__ __forceinline__ void finish_column(const Item& I, const Planes& P, const Poly& C, int turn, int i, int j, float (&v)[4],
+                                              uint32_t (&w)[4]) {
+    const int64_t to = static_cast<int64_t>(j) * I.ls + i;
+    if constexpr (KIND == kPoly) {
+        const half4 h = *reinterpret_cast<const half4*>(P.a + to), l = *reinterpret_cast<const half4*>(P.a + P.na + to);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(C.b, whole(h[e], l[e]), C.c * v[e]);
+    } else if constexpr (KIND == kApply || KIND == kResult) {
+        const half4 h = *reinterpret_cast<const half4*>(P.xt[turn] + to), l = *reinterpret_cast<const half4*>(P.xt[turn] + P.nt + to);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(C.a, whole(h[e], l[e]), v[e]);
+    }
+    if constexpr (KIND == kResult) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(v[e]);
+        return;
+    }
+    half4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        _Float16 a, b;
+        split(v[e], a, b);
+        hi[e] = a;
+        lo[e] = b;
+        w[e] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, a)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
+    }
+    _Float16* o = KIND == kGram ? P.a : KIND == kPoly ? P.b : P.xt[turn ^ 1];
+    const int64_t n = KIND == kApply ? P.nt : P.na;
+    *reinterpret_cast<half4*>(o + to) = hi;
+    *reinterpret_cast<half4*>(o + n + to) = lo;
+}
+
+// Four columns j .. j + 3 of row i from their words, in row order (X, or the mirror image of a tile off the diagonal).
+template <Kind KIND>
+__device__ __forceinline__ void finish_row(const Item& I, const Planes& P, int i, int j, const uint32_t (&w)[4]) {
+    half4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(w[e]));
+        lo[e] = __builtin_bit_cast(_Float16, static_cast<uint16_t>(w[e] >> 16));
+    }
+    _Float16* o = KIND == kGram ? P.a : KIND == kPoly ? P.b : P.x;
+    const int64_t n = KIND == kApply ? P.nx : P.na, at = static_cast<int64_t>(i) * (KIND == kApply ? I.ll : I.ls) + j;
+    *reinterpret_cast<half4*>(o + at) = hi;
+    *reinterpret_cast<half4*>(o + n + at) = lo;
+}
+
+// Four columns c .. c + 3 of row r of the result, or of the weight it updates.
+template <typename T>
+__device__ __forceinline__ void write_result(const Item& I, const Update& U, int r, int c, const uint32_t (&w)[4]) {
+    if (r >= I.rows || c >= I.cols) return;
+    const int n = min(4, I.cols - c);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(w[e]);
+    if (U.on) {
+        float* to = I.weight + static_cast<int64_t>(r) * I.ld_weight + c;
+        const float keep = 1.f - U.lr * U.decay;
+        const float scale = U.lr * sqrtf(fmaxf(1.f, static_cast<float>(I.rows) / static_cast<float>(I.cols)));
+        if (n == 4) {
+            float old[4];
+            load_as_f32<float, 4>(to, old);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = old[e] * keep - scale * v[e];
+            store_from_f32<float, 4>(to, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < n) to[e] = to[e] * keep - scale * v[e];
+        }
+    } else {
+        T* to = static_cast<T*>(I.dst) + static_cast<int64_t>(r) * I.ld_dst + c;
+        if (n == 4) {
+            store_from_f32<T, 4>(to, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (e < n) to[e] = static_cast<T>(v[e]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// tiles through LDS
+// ---------------------------------------------------------------------------------------------
 // One 16-byte copy per lane from global memory straight to LDS: the wavefront's 1 KiB lands in order from `to`.
 __device__ __forceinline__ void copy_to_lds(const _Float16* from, _Float16* to) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-constexpr int kBK = 64;                    // k per stage: a tile row is 128 bytes, 8 chunks of 16
+// Four wavefronts, two by two; two stages of 64 along k.  (Measured at 2048 x 2048, where it matters most: stages of 32,
+// three to five of them, or eight wavefronts: within 3 % of these.)
+constexpr int kWaves = 4, kBk = 64, kStages = 2;
 
-// Rows of a stage in LDS: chunk c of row r lies at place c ^ (r & 7), so that the 32 rows a wavefront reads at one c
-// spread over all banks.  The copy puts lane i at place i, so lane i fetches the chunk that belongs there.
-template <int ROWS, int WAVES>
-__device__ __forceinline__ void copy_rows(const _Float16* __restrict__ from, int64_t ld, _Float16* to) {
+// Rows of a stage in LDS, kBk halves each: the chunk of 16 bytes c of row r lies at place c ^ turn_of(r), so that the 16
+// rows that are read at one c in one cycle (256 bytes) lie in different banks.  A copy puts lane i at place i: lane i
+// fetches what belongs there.
+__device__ __forceinline__ int turn_of(int r) { return r >> 1 & 7; }
+
+// Copy number C of a wavefront's share of a plane of rows.
+__device__ __forceinline__ void copy_rows(const _Float16* __restrict__ from, int64_t ld, _Float16* to, int C) {
+    constexpr int kChunks = kBk / 8, kRows = kWave / kChunks;
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    static_assert(ROWS % (8 * WAVES) == 0, "whole copies");
-#pragma unroll
-    for (int i = 0; i < ROWS / (8 * WAVES); ++i) {
-        const int r0 = (i * WAVES + wave) * 8, r = r0 + lane / 8, c = (lane % 8) ^ (r & 7);
-        copy_to_lds(from + r * ld + c * 8, to + r0 * kBK);
-    }
+    const int r0 = (C * kWaves + wave) * kRows, r = r0 + lane / kChunks, c = (lane % kChunks) ^ turn_of(r);
+    copy_to_lds(from + r * ld + c * 8, to + r0 * kBk);
 }
 __device__ __forceinline__ half8 chunk_at(const _Float16* tile, int r, int c) {
-    return *reinterpret_cast<const half8*>(tile + r * kBK + ((c ^ (r & 7)) * 8));
+    return *reinterpret_cast<const half8*>(tile + r * kBk + ((c ^ turn_of(r)) * 8));
 }
 
-// Workgroup: a TM x TN tile of one product of one item; WM x WN wavefronts, each FM x FN blocks of 32 x 32.
-template <typename T, Kind KIND, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(kWave* WM* WN) void ortho_product(Items L, Update U, Poly C, int turn, _Float16* __restrict__ ws) {
-    constexpr int FM = TM / WM / 32, FN = TN / WN / 32, WAVES = WM * WN;
-    constexpr int kStage = (TM + TN) * kBK * 2;            // halves: P hi, P lo, Q hi, Q lo
-    extern __shared__ __align__(16) _Float16 lds[];
-    int b = blockIdx.x, k = 0;
-    for (;; ++k) {                                          // the grid is the sum of the items' tiles
-        const int mt = L.it[k].sp / TM, nt = (KIND == kGram || KIND == kPoly) ? L.it[k].sp / TN : L.it[k].lp / TN;
-        const int t = (KIND == kGram || KIND == kPoly) ? mt * (mt + 1) / 2 : mt * nt;
-        if (b < t) break;
-        b -= t;
-    }
-    const Item& I = L.it[k];
-    const Planes P = planes_of(I, ws);
-    int bi, bj;
-    if constexpr (KIND == kGram || KIND == kPoly) {
-        static_assert(KIND == kApply || KIND == kResult || TM == TN, "symmetric products have square tiles");
-        bj = static_cast<int>((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
-        while (bj * (bj + 1) / 2 > b) --bj;
-        while ((bj + 1) * (bj + 2) / 2 <= b) ++bj;
-        bi = b - bj * (bj + 1) / 2;                         // bi <= bj
-    } else {
-        const int nt = I.lp / TN;
-        bi = b / nt;
-        bj = b - bi * nt;
-    }
-    const int i0 = bi * TM, j0 = bj * TN;
-    const int K = KIND == kGram ? I.lp : I.sp;
-    const _Float16 *ph, *qh;
-    int64_t pn, qn;                                         // from the hi plane to the lo plane
-    if constexpr (KIND == kGram) { ph = qh = P.x; pn = qn = P.nx; }
-    else if constexpr (KIND == kPoly) { ph = qh = P.a; pn = qn = P.na; }
-    else { ph = P.b; pn = P.na; qh = P.xt[turn]; qn = P.nx; }
-    ph += static_cast<int64_t>(i0) * K;
-    qh += static_cast<int64_t>(j0) * K;
+// Halves of LDS of a stage: P hi, P lo, Q hi, Q lo.
+constexpr int stage_halves(int tile) { return 2 * tile * kBk * 2; }
+constexpr size_t lds_bytes(int tile) { return sizeof(_Float16) * stage_halves(tile) * kStages; }
 
-    auto fetch = [&](int k0, int stage) {
-        _Float16* s = lds + stage * kStage;
-        copy_rows<TM, WAVES>(ph + k0, K, s);
-        copy_rows<TM, WAVES>(ph + pn + k0, K, s + TM * kBK);
-        copy_rows<TN, WAVES>(qh + k0, K, s + 2 * TM * kBK);
-        copy_rows<TN, WAVES>(qh + qn + k0, K, s + (2 * TM + TN) * kBK);
+// Meets the other wavefronts once all but the last N of this wavefront's copies have landed (copies land in order) and its
+// reads are done.  __syncthreads() would wait for every copy, those of the stages ahead too.
+template <int N>
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Orders a wavefront's own writes of LDS before its reads (the unit serves them in order).
+__device__ __forceinline__ void wave_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Asks the scheduler for PRODUCTS matrix instructions with READS reads of LDS, then COPIES copies to LDS spread between
+// them.  A copy occupies the address unit for some 16 cycles, which four wavefronts share: issued in one go at the head of
+// a stage, they kept the matrix cores waiting for a third of the time.
+template <int PRODUCTS, int READS, int COPIES, int X = 0>
+__device__ __forceinline__ void interleave() {
+    constexpr int kOthers = READS + COPIES;
+    if constexpr (X < kOthers) {
+        constexpr int n = PRODUCTS * (X + 1) / kOthers - PRODUCTS * X / kOthers;
+        if constexpr (n > 0) __builtin_amdgcn_sched_group_barrier(0x008, n, 0);
+        __builtin_amdgcn_sched_group_barrier(X < READS ? 0x100 : 0x010, 1, 0);
+        interleave<PRODUCTS, READS, COPIES, X + 1>();
+    }
+}
+
+// Workgroup: a TILE x TILE tile of one product of one item; each wavefront a quarter of it, N x N blocks of 32 x 32;
+// kStages of kBk along k in LDS, of which all but the one at work are being filled.
+template <typename T, Kind KIND, int TILE>
+__global__ __launch_bounds__(kWave* kWaves) void ortho_product(const Items* __restrict__ list, Update U, Poly C, int turn, _Float16* __restrict__ ws) {
+    constexpr int N = TILE / 64, kStage = stage_halves(TILE), kPlane = TILE * kBk;
+    constexpr int kCopies = kStage / 8 / (kWave * kWaves);  // copies of a wavefront per stage
+    constexpr int kSteps = kBk / 16, kShare = kCopies / kSteps, kPer = kCopies / 4;            // ... per step, per plane
+    static_assert(kShare * kSteps == kCopies && kPer * 4 == kCopies, "whole copies, equal shares");
+    extern __shared__ __align__(16) _Float16 lds[];
+    const Tile t = tile_of<KIND, TILE>(*list);
+    const Item I = list->it[t.item];
+    const Planes P = planes_of(I, ws);
+    const Operands O = operands_of<KIND>(I, P, t, turn);
+    auto copy = [&](int k0, int stage, int c) {             // copy c of a stage
+        const _Float16* from = c < kPer ? O.p : c < 2 * kPer ? O.p + O.pn : c < 3 * kPer ? O.q : O.q + O.qn;
+        copy_rows(from + k0, O.ld, lds + stage * kStage + c / kPer * kPlane, c % kPer);
     };
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const int wi = wave / WN * (TM / WM), wj = wave % WN * (TN / WN);
+    const int wi = wave / 2 * (TILE / 2), wj = wave % 2 * (TILE / 2);
     const int lr = lane % 32, lk = lane / 32;
-    f32x16 main_sum[FM][FN], lo_sum[FM][FN];
+    f32x16 main_sum[N][N], lo_sum[N][N];
 #pragma unroll
-    for (int m = 0; m < FM; ++m)
+    for (int m = 0; m < N; ++m)
 #pragma unroll
-        for (int n = 0; n < FN; ++n)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) main_sum[m][n][e] = lo_sum[m][n][e] = 0.f;
-    fetch(0, 0);
-    for (int k0 = 0, stage = 0; k0 < K; k0 += kBK, stage ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0);                      // this wavefront's copies have landed ...
-        __syncthreads();                                    // ... and everyone's; the other stage is read out
-        if (k0 + kBK < K) fetch(k0 + kBK, stage ^ 1);
+    struct Frags { half8 ah[N], al[N], bh[N], bl[N]; };
+    auto read = [&](const _Float16* s, int q, Frags& f) {
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+            f.ah[m] = chunk_at(s, wi + m * 32 + lr, 2 * q + lk);
+            f.al[m] = chunk_at(s + kPlane, wi + m * 32 + lr, 2 * q + lk);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            f.bh[n] = chunk_at(s + 2 * kPlane, wj + n * 32 + lr, 2 * q + lk);
+            f.bl[n] = chunk_at(s + 3 * kPlane, wj + n * 32 + lr, 2 * q + lk);
+        }
+    };
+    const int last = O.K - kBk;                              // past the end the last stage is fetched again, for nobody
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s)
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) copy(min(s * kBk, last), s, c);
+    int stage = 0;
+    for (int k0 = 0; k0 < O.K; k0 += kBk) {
+        // stage k0 has landed, everyone's part; the stage before is read out.  The kStages - 2 after k0 may be under way.
+        meet<(kStages - 2) * kCopies>();
         const _Float16* s = lds + stage * kStage;
+        const int next = min(k0 + (kStages - 1) * kBk, last), into = stage == 0 ? kStages - 1 : stage - 1;
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        Frags f[2];
+        read(s, 0, f[0]);
 #pragma unroll
-        for (int q = 0; q < kBK / 16; ++q) {
-            half8 ah[FM], al[FM], bh[FN], bl[FN];
+        for (int q = 0; q < kSteps; ++q) {
+            if (q + 1 < kSteps) read(s, q + 1, f[(q + 1) & 1]);
 #pragma unroll
-            for (int m = 0; m < FM; ++m) {
-                ah[m] = chunk_at(s, wi + m * 32 + lr, 2 * q + lk);
-                al[m] = chunk_at(s + TM * kBK, wi + m * 32 + lr, 2 * q + lk);
-            }
+            for (int c = 0; c < kShare; ++c) copy(next, into, q * kShare + c);
+            const Frags& g = f[q & 1];
 #pragma unroll
-            for (int n = 0; n < FN; ++n) {
-                bh[n] = chunk_at(s + 2 * TM * kBK, wj + n * 32 + lr, 2 * q + lk);
-                bl[n] = chunk_at(s + (2 * TM + TN) * kBK, wj + n * 32 + lr, 2 * q + lk);
-            }
+            for (int m = 0; m < N; ++m)
 #pragma unroll
-            for (int m = 0; m < FM; ++m)
-#pragma unroll
-                for (int n = 0; n < FN; ++n) {
-                    main_sum[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[m], bh[n], main_sum[m][n], 0, 0, 0);
-                    lo_sum[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[m], bl[n], lo_sum[m][n], 0, 0, 0);
-                    lo_sum[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[m], bh[n], lo_sum[m][n], 0, 0, 0);
+                for (int n = 0; n < N; ++n) {
+                    main_sum[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.ah[m], g.bh[n], main_sum[m][n], 0, 0, 0);
+                    lo_sum[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.ah[m], g.bl[n], lo_sum[m][n], 0, 0, 0);
                 }
+#pragma unroll
+            for (int m = 0; m < N; ++m)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    lo_sum[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(g.al[m], g.bh[n], lo_sum[m][n], 0, 0, 0);
+        }
+        // order: the first step's reads, then each step's matrix instructions with the next step's reads between them
+        constexpr int kReads = 4 * N, kProducts = 3 * N * N;
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+#pragma unroll
+        for (int q = 0; q + 1 < kSteps; ++q) interleave<kProducts, kReads, kShare>();
+        interleave<kProducts, 0, kShare>();
+    }
+    meet<0>();                                              // no copy is under way, nobody reads a stage any more
+    // The sums go through LDS, a wavefront's block at a time, so that what lies along memory is read and written in runs
+    // of its whole side: buf[j][i].  (Straight from the registers, 16 bytes of a line at a time, this cost as much as a
+    // third of the products.)  Element e of a block: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.
+    constexpr int kSide = N * 32, kRow = kSide + 4;
+    static_assert(kWaves * kSide * kRow * sizeof(uint32_t) <= lds_bytes(TILE), "fits the stages");
+    uint32_t* buf = reinterpret_cast<uint32_t*>(lds) + wave * kSide * kRow;
+#pragma unroll
+    for (int m = 0; m < N; ++m)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t* to = buf + (n * 32 + lr) * kRow + m * 32 + 8 * g + 4 * lk;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    to[e] = __float_as_uint(__builtin_fmaf(lo_sum[m][n][4 * g + e], 1.f / kLo, main_sum[m][n][4 * g + e]));
+            }
+    wave_lds();
+    const bool tall = I.rows > I.cols;
+#pragma unroll 4
+    for (int x = lane; x < kSide * kSide / 4; x += kWave) {
+        const int i = x % (kSide / 4) * 4, j = x / (kSide / 4);
+        uint32_t w[4];
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(buf[j * kRow + i + e]);
+        finish_column<KIND>(I, P, C, turn, t.i0 + wi + i, t.j0 + wj + j, v, w);
+        if (KIND == kResult && tall) {
+            write_result<T>(I, U, t.j0 + wj + j, t.i0 + wi + i, w);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) buf[j * kRow + i + e] = w[e];
         }
     }
-    // element e of a block: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+    if (KIND == kResult ? tall : symmetric(KIND) && t.i0 == t.j0) return;      // (a tile on the diagonal is its own mirror image)
+    wave_lds();
+#pragma unroll 4
+    for (int x = lane; x < kSide * kSide / 4; x += kWave) {
+        const int j = x % (kSide / 4) * 4, i = x / (kSide / 4);
+        uint32_t w[4];
 #pragma unroll
-    for (int m = 0; m < FM; ++m)
+        for (int e = 0; e < 4; ++e) w[e] = buf[(j + e) * kRow + i];
+        if constexpr (KIND == kResult) write_result<T>(I, U, t.i0 + wi + i, t.j0 + wj + j, w);
+        else finish_row<KIND>(I, P, t.i0 + wi + i, t.j0 + wj + j, w);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// tiles of 32 for small matrices
+// ---------------------------------------------------------------------------------------------
+constexpr int kSmall = 32, kSmallWaves = 8, kSmallAhead = 4;
+
+// Workgroup: a 32 x 32 tile; wavefront w takes its share of the steps of 16 along k, kSmallAhead of them in flight.
+template <typename T, Kind KIND>
+__global__ __launch_bounds__(kWave* kSmallWaves) void ortho_product_small(const Items* __restrict__ list, Update U, Poly C, int turn, _Float16* __restrict__ ws) {
+    __shared__ float part[kSmallWaves][kSmall][kSmall + 1];
+    const Tile t = tile_of<KIND, kSmall>(*list);
+    const Item I = list->it[t.item];
+    const Planes P = planes_of(I, ws);
+    const Operands O = operands_of<KIND>(I, P, t, turn);
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, lr = lane % 32, lk = lane / 32;
+    const _Float16* p = O.p + static_cast<int64_t>(lr) * O.ld + lk * 8;
+    const _Float16* q = O.q + static_cast<int64_t>(lr) * O.ld + lk * 8;
+    f32x16 main_sum, lo_sum;
 #pragma unroll
-        for (int n = 0; n < FN; ++n)
+    for (int e = 0; e < 16; ++e) main_sum[e] = lo_sum[e] = 0.f;
+    const int steps = O.K / 16;
+    for (int s0 = wave; s0 < steps; s0 += kSmallWaves * kSmallAhead) {
+        half8 ah[kSmallAhead], al[kSmallAhead], bh[kSmallAhead], bl[kSmallAhead];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int i = i0 + wi + m * 32 + 8 * (e / 4) + 4 * lk + e % 4, j = j0 + wj + n * 32 + lr;
-                float v = __builtin_fmaf(lo_sum[m][n][e], 1.f / kLo, main_sum[m][n][e]);
-                _Float16 hi, lo;
-                if constexpr (KIND == kGram || KIND == kPoly) {
-                    const int64_t at = static_cast<int64_t>(i) * I.sp + j, to = static_cast<int64_t>(j) * I.sp + i;
-                    if constexpr (KIND == kPoly) v = __builtin_fmaf(C.b, whole(P.a[at], P.a[P.na + at]), C.c * v);
-                    split(v, hi, lo);
-                    _Float16* o = KIND == kGram ? P.a : P.b;
-                    o[at] = hi;
-                    o[P.na + at] = lo;
-                    if (bi != bj) { o[to] = hi; o[P.na + to] = lo; }
-                } else {
-                    const int64_t at = static_cast<int64_t>(i) * I.lp + j, to = static_cast<int64_t>(j) * I.sp + i;
-                    v = __builtin_fmaf(C.a, whole(P.x[at], P.x[P.nx + at]), v);
-                    if constexpr (KIND == kApply) {
-                        split(v, hi, lo);
-                        P.x[at] = hi;
-                        P.x[P.nx + at] = lo;
-                        P.xt[turn ^ 1][to] = hi;
-                        P.xt[turn ^ 1][P.nx + to] = lo;
-                    } else {
-                        const bool tall = I.rows > I.cols;
-                        const int r = tall ? j : i, c = tall ? i : j;
-                        if (r < I.rows && c < I.cols) {
-                            if (U.on) {
-                                float* w = I.weight + static_cast<int64_t>(r) * I.ld_weight + c;
-                                const float scale = sqrtf(fmaxf(1.f, static_cast<float>(I.rows) / static_cast<float>(I.cols)));
-                                *w = *w * (1.f - U.lr * U.decay) - (U.lr * scale) * v;
-                            } else {
-                                static_cast<T*>(I.dst)[static_cast<int64_t>(r) * I.ld_dst + c] = static_cast<T>(v);
-                            }
-                        }
-                    }
-                }
-            }
+        for (int a = 0; a < kSmallAhead; ++a) {
+            const int k = min(s0 + a * kSmallWaves, steps - 1) * 16;
+            ah[a] = *reinterpret_cast<const half8*>(p + k);
+            al[a] = *reinterpret_cast<const half8*>(p + O.pn + k);
+            bh[a] = *reinterpret_cast<const half8*>(q + k);
+            bl[a] = *reinterpret_cast<const half8*>(q + O.qn + k);
+        }
+#pragma unroll
+        for (int a = 0; a < kSmallAhead; ++a) {
+            if (s0 + a * kSmallWaves >= steps) break;       // the same for the whole wavefront
+            main_sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[a], bh[a], main_sum, 0, 0, 0);
+            lo_sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[a], bl[a], lo_sum, 0, 0, 0);
+            lo_sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[a], bh[a], lo_sum, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) part[wave][lr][8 * (e / 4) + 4 * lk + e % 4] = __builtin_fmaf(lo_sum[e], 1.f / kLo, main_sum[e]);
+    __syncthreads();
+    // 256 threads: four rows of a column each, then four columns of a row
+    const int u = threadIdx.x / 8, f = threadIdx.x % 8 * 4;
+    const bool active = threadIdx.x < 256, tall = I.rows > I.cols;
+    uint32_t w[4];
+    if (active) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = part[0][u][f + e];
+#pragma unroll
+            for (int x = 1; x < kSmallWaves; ++x) v[e] += part[x][u][f + e];
+        }
+        finish_column<KIND>(I, P, C, turn, t.i0 + f, t.j0 + u, v, w);
+        if (KIND == kResult && tall) write_result<T>(I, U, t.j0 + u, t.i0 + f, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[0][u][f + e] = __uint_as_float(w[e]);
+    }
+    if (KIND == kResult ? tall : symmetric(KIND) && t.i0 == t.j0) return;
+    __syncthreads();
+    if (!active) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(part[0][f + e][u]);
+    if constexpr (KIND == kResult) write_result<T>(I, U, t.i0 + u, t.j0 + f, w);
+    else finish_row<KIND>(I, P, t.i0 + u, t.j0 + f, w);
 }
 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-constexpr int kTile = 64;
-constexpr size_t kLds = static_cast<size_t>(2 * kTile) * kBK * 2 * sizeof(_Float16) * 2;
+constexpr int64_t kMaxTiles = 1LL << 30;
 
-int padded(int v) { return (v + kTile - 1) / kTile * kTile; }
+int padded(int v, int unit) { return (v + unit - 1) / unit * unit; }
 
-// Sides of the items of one turn; halves of workspace they need.
-int64_t lay_out(const cbm_ortho_item* items, int n, Items& L) {
-    int64_t halves = 0;
+int64_t tiles_of(const Items& L, bool square, int tile) {
+    int64_t n = 0;
+    for (int i = 0; i < L.n; ++i) {
+        const int64_t s = (L.it[i].sp + tile - 1) / tile, l = (L.it[i].lp + tile - 1) / tile;
+        n += square ? s * (s + 1) / 2 : s * l;
+    }
+    return n;
+}
+
+// Tile size of a launch: a larger tile fetches less for its work, but wants half the chip's 256 CUs to have one.
+// Measured, the other choice in brackets: 136 symmetric tiles of 128 (side 2048) 49 us [58]; 80 of them, as 288 tiles of
+// 64 (8 x 512 x 1024) 17.6 us [25.7]; 96 tiles of 64 (333 x 1001) as 352 of 32 11.4 us [11.2].
+constexpr int kFullGrid = 128;
+int choose(const Items& L, bool square) {
+    if (tiles_of(L, square, 128) >= kFullGrid) return 128;
+    return tiles_of(L, square, 64) >= kFullGrid ? 64 : 32;
+}
+
+// Sides of the items of one turn; halves of workspace they need.  All sides are padded to the larger tile in use.
+struct Choice { int square, wide; };
+int64_t lay_out(const cbm_ortho_item* items, int n, Items& L, Choice& choice) {
     L.n = 0;
     for (int i = 0; i < n; ++i) {
         const cbm_ortho_item& s = items[i];
@@ -331,45 +643,76 @@ int64_t lay_out(const cbm_ortho_item* items, int n, Items& L) {
         d.src = s.src; d.dst = s.dst; d.weight = s.weight; d.momentum = s.momentum;
         d.ld_src = s.ld_src; d.ld_dst = s.ld_dst; d.ld_weight = s.ld_weight; d.ld_momentum = s.ld_momentum;
         d.rows = s.rows; d.cols = s.cols;
-        d.sp = padded(std::min(s.rows, s.cols));
-        d.lp = padded(std::max(s.rows, s.cols));
+        d.sp = std::min(s.rows, s.cols);
+        d.lp = std::max(s.rows, s.cols);
+        d.norm_blocks = std::max<int64_t>(1, std::min<int64_t>({kNormBlocks, (s.rows + 3) / 4, static_cast<int64_t>(s.rows) * s.cols / 1024}));
+    }
+    choice = {choose(L, true), choose(L, false)};
+    const int unit = std::max(choice.square, choice.wide);
+    int64_t halves = 0;
+    for (int i = 0; i < L.n; ++i) {
+        Item& d = L.it[i];
+        d.sp = padded(d.sp, unit);
+        d.lp = padded(d.lp, unit);
+        d.ls = d.sp;                                        // (rows 128 bytes further apart, off powers of two: no gain)
+        d.ll = d.lp;
         d.base = halves;
-        halves += item_halves(d.sp, d.lp);
+        halves += item_halves(d);
+    }
+    int ends[kGrids] = {};
+    for (int i = 0; i < kMaxItems; ++i) {
+        if (i < L.n) {
+            const int64_t s = L.it[i].sp, l = L.it[i].lp, q = s / choice.square;
+            if (tiles_of(L, false, 32) <= kMaxTiles) {
+                ends[kSplitGrid] += static_cast<int>(((s + 63) / 64) * ((l + 63) / 64));
+                ends[kSquareGrid] += static_cast<int>(q * (q + 1) / 2);
+                ends[kWideGrid] += static_cast<int>((s / choice.wide) * (l / choice.wide));
+            }
+        }
+        for (int g = 0; g < kGrids; ++g) L.ends[g][i] = i < L.n ? ends[g] : INT_MAX;
     }
     return halves;
 }
 
 constexpr int64_t kNormBytes = static_cast<int64_t>(kMaxItems) * kNormBlocks * sizeof(double);
+constexpr int64_t kListBytes = 4096;
+static_assert(sizeof(Items) <= kListBytes, "the list");
+
+template <typename T, Kind KIND>
+int launch_product(int tile, const Items& L, const Items* list, const Update& U, const Poly& C, int turn, _Float16* ws, hipStream_t st) {
+    const unsigned blocks = static_cast<unsigned>(tiles_of(L, symmetric(KIND), tile));
+    if (tile == 128) {
+        hipLaunchKernelGGL((ortho_product<T, KIND, 128>), dim3(blocks), dim3(kWave * kWaves), lds_bytes(128), st, list, U, C, turn, ws);
+    } else if (tile == 64) {
+        hipLaunchKernelGGL((ortho_product<T, KIND, 64>), dim3(blocks), dim3(kWave * kWaves), lds_bytes(64), st, list, U, C, turn, ws);
+    } else {
+        hipLaunchKernelGGL((ortho_product_small<T, KIND>), dim3(blocks), dim3(kWave * kSmallWaves), 0, st, list, U, C, turn, ws);
+    }
+    return check_launch();
+}
 
 template <typename T>
 int run_turn(const cbm_ortho_item* items, int n, const Update& U, int steps, const Poly& C, float eps, void* workspace, hipStream_t st) {
     Items L;
-    lay_out(items, n, L);
+    Choice choice;
+    lay_out(items, n, L, choice);
     if (L.n == 0) return CBM_OK;
-    double* partial = static_cast<double*>(workspace);
-    _Float16* ws = reinterpret_cast<_Float16*>(static_cast<char*>(workspace) + kNormBytes);
-    int64_t square = 0, wide = 0, tiles64 = 0;
-    for (int i = 0; i < L.n; ++i) {
-        const int64_t s = L.it[i].sp / kTile, l = L.it[i].lp / kTile;
-        square += s * (s + 1) / 2;
-        wide += s * l;
-        tiles64 += static_cast<int64_t>(L.it[i].sp / 64) * (L.it[i].lp / 64);
-    }
-    if (wide > (1LL << 30) || square > (1LL << 30)) return CBM_ERR_SHAPE;
-    hipLaunchKernelGGL(ortho_norms<T>, dim3(kNormBlocks, L.n), dim3(256), 0, st, L, U, partial);
+    Items* list = static_cast<Items*>(workspace);
+    double* partial = reinterpret_cast<double*>(static_cast<char*>(workspace) + kListBytes);
+    _Float16* ws = reinterpret_cast<_Float16*>(static_cast<char*>(workspace) + kListBytes + kNormBytes);
+    if (tiles_of(L, false, 32) > kMaxTiles) return CBM_ERR_SHAPE;
+    int norm_blocks = 1;
+    for (int i = 0; i < L.n; ++i) norm_blocks = std::max(norm_blocks, L.it[i].norm_blocks);
+    hipLaunchKernelGGL(ortho_norms<T>, dim3(norm_blocks, L.n), dim3(256), 0, st, L, U, list, partial);
     if (int rc = check_launch()) return rc;
-    hipLaunchKernelGGL(ortho_split<T>, dim3(static_cast<unsigned>(tiles64)), dim3(256), 0, st, L, U, partial, eps, ws);
+    hipLaunchKernelGGL(ortho_split<T>, dim3(static_cast<unsigned>(tiles_of(L, false, 64))), dim3(256), 0, st, list, U, partial, eps, ws);
     if (int rc = check_launch()) return rc;
     for (int t = 0; t < steps; ++t) {
-        hipLaunchKernelGGL((ortho_product<T, kGram, kTile, kTile, 2, 2>), dim3(static_cast<unsigned>(square)), dim3(256), kLds, st, L, U, C, t & 1, ws);
-        if (int rc = check_launch()) return rc;
-        hipLaunchKernelGGL((ortho_product<T, kPoly, kTile, kTile, 2, 2>), dim3(static_cast<unsigned>(square)), dim3(256), kLds, st, L, U, C, t & 1, ws);
-        if (int rc = check_launch()) return rc;
-        if (t + 1 < steps)
-            hipLaunchKernelGGL((ortho_product<T, kApply, kTile, kTile, 2, 2>), dim3(static_cast<unsigned>(wide)), dim3(256), kLds, st, L, U, C, t & 1, ws);
-        else
-            hipLaunchKernelGGL((ortho_product<T, kResult, kTile, kTile, 2, 2>), dim3(static_cast<unsigned>(wide)), dim3(256), kLds, st, L, U, C, t & 1, ws);
-        if (int rc = check_launch()) return rc;
+        if (int rc = launch_product<T, kGram>(choice.square, L, list, U, C, t & 1, ws, st)) return rc;
+        if (int rc = launch_product<T, kPoly>(choice.square, L, list, U, C, t & 1, ws, st)) return rc;
+        const int rc = t + 1 < steps ? launch_product<T, kApply>(choice.wide, L, list, U, C, t & 1, ws, st)
+                                     : launch_product<T, kResult>(choice.wide, L, list, U, C, t & 1, ws, st);
+        if (rc) return rc;
     }
     return CBM_OK;
 }
@@ -405,9 +748,10 @@ int64_t cbm_ortho_workspace_bytes(const cbm_ortho_item* items, int32_t n) {
     int64_t most = 0;
     for (int i = 0; i < n; i += kMaxItems) {
         Items L;
-        most = std::max(most, lay_out(items + i, std::min(kMaxItems, n - i), L));
+        Choice choice;
+        most = std::max(most, lay_out(items + i, std::min(kMaxItems, n - i), L, choice));
     }
-    return most ? kNormBytes + most * static_cast<int64_t>(sizeof(_Float16)) : 0;
+    return most ? kListBytes + kNormBytes + most * static_cast<int64_t>(sizeof(_Float16)) : 0;
 }
 
 int cbm_orthogonalise(const cbm_ortho_item* items, int32_t n, int32_t steps, float a, float b, float c, float eps, int32_t dtype,
