@@ -1,7 +1,10 @@
 """What the dense operators (``norm``, ``labels``, ``optim``) share: element types, layout checks, launches."""
 from __future__ import annotations
 
+import functools
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from .cbm import _require_gpu, _stream  # noqa: F401  (the streams and the no-GPU error are the multiply's)
 
@@ -54,6 +57,16 @@ def grad_rows(g, rows, width):
 
 def ld(t):
     return t.stride(0) if t.size(0) > 1 else max(t.size(1), 1)
+
+
+def once(backward):
+    """``once_differentiable`` where a graph of the gradient is asked for; its 10 us are spent nowhere else."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def ptr(t):

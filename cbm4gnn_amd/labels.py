@@ -11,13 +11,13 @@ Calls on CPU tensors are staged through the GPU, as the multiply's are.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._dense import DTYPES, _require_gpu, _stream, check_dtype, check_int32, grad_rows, ld, on_device, ptr, rows_view
+from ._dense import DTYPES, _require_gpu, _stream, check_dtype, check_int32, ld, on_device, once, ptr, rows_view
 
 __all__ = ["LabelScores", "label_log_probs"]
 
@@ -31,22 +31,26 @@ class LabelScores(NamedTuple):
     top_index: Optional[torch.Tensor]
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_floats(rows, classes, top, dtype):
+    return _lib.hip_lib().cbm_label_scores_workspace_floats(rows, classes, top, dtype)
+
+
 def _forward(z, labels, entropy, top, ignore_index, keep):
     rows, classes = z.shape
-    lib = _lib.hip_lib()
-    dev = z.device
-    f32 = dict(dtype=torch.float32, device=dev)
-    logp = torch.empty(rows, **f32) if labels is not None else None
-    ent = torch.empty(rows, **f32) if entropy else None
-    top_logp = torch.empty((rows, top), **f32) if top else None
+    dev, dt, f32 = z.device, DTYPES[z.dtype], torch.float32
+    logp = torch.empty(rows, dtype=f32, device=dev) if labels is not None else None
+    ent = torch.empty(rows, dtype=f32, device=dev) if entropy else None
+    top_logp = torch.empty((rows, top), dtype=f32, device=dev) if top else None
     top_index = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty((rows, 2), **f32) if keep else None
-    floats = lib.cbm_label_scores_workspace_floats(rows, classes, top, DTYPES[z.dtype])
-    ws = torch.empty(floats, **f32) if floats else None
+    stats = torch.empty((rows, 2), dtype=f32, device=dev) if keep else None
+    floats = _workspace_floats(rows, classes, top, dt)
+    ws = torch.empty(floats, dtype=f32, device=dev) if floats else None
     with on_device(dev):
-        rc = lib.cbm_label_scores(ptr(z), ptr(labels), ptr(logp), ptr(ent), ptr(top_logp), ptr(top_index), ptr(stats), ptr(ws), rows,
-                                  classes, top, ld(z), ignore_index, DTYPES[z.dtype], _stream(dev))
-    _lib.check(rc, "cbm_label_scores")
+        rc = _lib.hip_lib().cbm_label_scores(ptr(z), ptr(labels), ptr(logp), ptr(ent), ptr(top_logp), ptr(top_index), ptr(stats), ptr(ws),
+                                             rows, classes, top, ld(z), ignore_index, dt, _stream(dev))
+    if rc:
+        _lib.check(rc, "cbm_label_scores")
     return logp, ent, top_logp, top_index, stats
 
 
@@ -62,17 +66,19 @@ class _LabelScores(torch.autograd.Function):
         return logp, ent, top_logp, top_index
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, g_logp, g_ent, g_top, _):
         z, labels, stats, ent, top_index = ctx.saved_tensors
         rows, classes = z.shape
+        dev, dt = z.device, DTYPES[z.dtype]
         flat = [g if g is None or g.is_contiguous() else g.contiguous() for g in (g_logp, g_ent, g_top)]
-        grad = torch.empty((rows, classes), dtype=z.dtype, device=z.device)
-        with on_device(z.device):
+        grad = torch.empty((rows, classes), dtype=z.dtype, device=dev)
+        with on_device(dev):
             rc = _lib.hip_lib().cbm_label_scores_backward(
-                ptr(z), ptr(labels), ptr(stats), ptr(ent), ptr(top_index), *map(ptr, flat), ptr(grad), rows, classes, ctx.top, ld(z),
-                classes, ctx.ignore_index, DTYPES[z.dtype], _stream(z.device))
-        _lib.check(rc, "cbm_label_scores_backward")
+                ptr(z), ptr(labels), ptr(stats), ptr(ent), ptr(top_index), ptr(flat[0]), ptr(flat[1]), ptr(flat[2]), ptr(grad), rows,
+                classes, ctx.top, ld(z), classes, ctx.ignore_index, dt, _stream(dev))
+        if rc:
+            _lib.check(rc, "cbm_label_scores_backward")
         return grad, None, None, None, None
 
 
@@ -116,7 +122,8 @@ def label_log_probs(logits, labels=None, *, entropy=False, top=0, ignore_index=-
                             ignore_index=ignore_index)
         return LabelScores(*(None if t is None else t.to(logits.device) for t in r))
     if labels is not None:
-        labels = labels.reshape(rows).to(torch.int64).contiguous()
+        if labels.dtype != torch.int64 or labels.dim() != 1 or not labels.is_contiguous():
+            labels = labels.reshape(rows).to(torch.int64).contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         parts = _LabelScores.apply(z, labels, bool(entropy), top, ignore_index)
     else:

@@ -18,10 +18,9 @@ import functools
 import numpy as np
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._dense import DTYPES, _require_gpu, _stream, check_dtype, check_int32, grad_rows, ld, on_device, ptr, rows_view
+from ._dense import DTYPES, _require_gpu, _stream, check_dtype, check_int32, grad_rows, ld, on_device, once, ptr, rows_view
 
 __all__ = ["GraphBatch", "group_norm", "GroupNorm"]
 
@@ -93,54 +92,51 @@ class GraphBatch:
         return st
 
 
-def _forward(x, weight, bias, batch, groups, eps, act, keep):
-    m = rows_view(x, "x")
-    rows, ch = m.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    lib = _lib.hip_lib()
-    dt = DTYPES[x.dtype]
-    b = C.byref(batch)
+def _forward(x, m, weight, bias, batch, groups, eps, act, keep):
+    ch, dev, dt, f32 = m.size(1), x.device, DTYPES[x.dtype], torch.float32
+    lib, b = _lib.hip_lib(), C.byref(batch)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     mean = rstd = None
     if keep:
-        mean = torch.empty((batch.samples, groups), dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
+        mean = torch.empty((batch.samples, groups), dtype=f32, device=dev)
+        rstd = torch.empty((batch.samples, groups), dtype=f32, device=dev)
     floats = lib.cbm_group_norm_workspace_floats(b, ch, groups, dt, 0)
-    ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-    with on_device(x.device):
+    ws = torch.empty(floats, dtype=f32, device=dev) if floats else None
+    with on_device(dev):
         rc = lib.cbm_group_norm_forward(b, ptr(m), ptr(y), ptr(weight), ptr(bias), ptr(mean), ptr(rstd), ptr(ws), ch, groups,
-                                        ld(m), ch, eps, act, dt, _stream(x.device))
-    _lib.check(rc, "cbm_group_norm_forward")
+                                        ld(m), ch, eps, act, dt, _stream(dev))
+    if rc:
+        _lib.check(rc, "cbm_group_norm_forward")
     return y, mean, rstd
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, batch, groups, eps, act):
-        y, mean, rstd = _forward(x, weight, bias, batch, groups, eps, act, True)
+        y, mean, rstd = _forward(x, rows_view(x, "x"), weight, bias, batch, groups, eps, act, True)
         ctx.save_for_backward(x, weight, bias, mean, rstd)
         ctx.batch, ctx.groups, ctx.act = batch, groups, act
         return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         x, weight, bias, mean, rstd = ctx.saved_tensors
         m = rows_view(x, "x")
         rows, ch = m.shape
         g = grad_rows(dy, rows, ch)
-        need = ctx.needs_input_grad
-        lib = _lib.hip_lib()
-        dt = DTYPES[x.dtype]
-        b = C.byref(ctx.batch)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-        dw = torch.empty_like(weight) if need[1] else None
-        db = torch.empty_like(bias) if need[2] else None
+        need, dev, dt, f32 = ctx.needs_input_grad, x.device, DTYPES[x.dtype], torch.float32
+        lib, b = _lib.hip_lib(), C.byref(ctx.batch)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+        dw = torch.empty(ch, dtype=f32, device=dev) if need[1] else None
+        db = torch.empty(ch, dtype=f32, device=dev) if need[2] else None
         floats = lib.cbm_group_norm_workspace_floats(b, ch, ctx.groups, dt, 1)
-        ws = torch.empty(floats, dtype=torch.float32, device=x.device) if floats else None
-        with on_device(x.device):
+        ws = torch.empty(floats, dtype=f32, device=dev) if floats else None
+        with on_device(dev):
             rc = lib.cbm_group_norm_backward(b, ptr(m), ptr(g), ptr(dx), ptr(weight), ptr(bias), ptr(mean), ptr(rstd), ptr(dw), ptr(db),
-                                             ptr(ws), ch, ctx.groups, ld(m), ld(g), ch, ctx.act, dt, _stream(x.device))
-        _lib.check(rc, "cbm_group_norm_backward")
+                                             ptr(ws), ch, ctx.groups, ld(m), ld(g), ch, ctx.act, dt, _stream(dev))
+        if rc:
+            _lib.check(rc, "cbm_group_norm_backward")
         return dx, dw, db, None, None, None, None
 
 
@@ -186,7 +182,7 @@ def group_norm(x, groups, weight=None, bias=None, *, graphs=None, eps=1e-5, acti
             raise ValueError(f"x has {x.size(0)} rows, the batch has {graphs.n_nodes} nodes")
     _check_channel(weight, "weight", ch, x.device)
     _check_channel(bias, "bias", ch, x.device)
-    rows_view(x, "x")
+    m = rows_view(x, "x")
     samples = graphs.n_graphs if graphs is not None else 1 if x.dim() == 2 else x.size(0)
     if samples * groups > 1 << 30:
         raise ValueError("graphs times groups: at most 2^30")
@@ -201,7 +197,7 @@ def group_norm(x, groups, weight=None, bias=None, *, graphs=None, eps=1e-5, acti
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _GroupNorm.apply(x, weight, bias, batch, groups, eps, act)
-    return _forward(x, weight, bias, batch, groups, eps, act, False)[0]
+    return _forward(x, m, weight, bias, batch, groups, eps, act, False)[0]
 
 
 class GroupNorm(nn.Module):
