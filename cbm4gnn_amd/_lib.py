@@ -118,6 +118,7 @@ class CbmOrthoItem(C.Structure):
 
 
 CBM_ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+CBM_NORM_MAX_GRAPHS, CBM_NORM_MAX_PAIRS = 1 << 21, 1 << 25
 CBM_LABELS_MAX_TOP = 32
 CBM_LABELS_MAX_CLASSES = 64 * 1024 * 8 * 4
 CBM_ORTHO_MAX_ITEMS = 24

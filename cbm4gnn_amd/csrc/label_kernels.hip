@@ -570,6 +570,64 @@ int check_labels(int rows, int classes, int top, int64_t ld, int dtype) {
 
 unsigned narrow_blocks(int rows, int L) { return static_cast<unsigned>((static_cast<int64_t>(rows) * L + kThreads - 1) / kThreads); }
 
+// Rows of one launch: a grid holds fewer than 2^32 threads along one dimension.
+int rows_at_once(int classes) { return classes <= kNarrowClasses ? 1 << 25 : 1 << 21; }      // 64 and 1024 threads a row at most
+
+// The scores of some rows, with s (of the whole call) for wide ones.
+int score_rows(const void* logits, const Outputs& O, float* workspace, int rows, int64_t ld, const Splits& s, int dtype, hipStream_t st) {
+    const int classes = O.classes;
+    if (classes <= kNarrowClasses) {
+#define NARROW(T, V, L, NV)                                                                                                  \
+    if (O.entropy || O.top > 0)                                                                                                \
+        hipLaunchKernelGGL((label_scores_narrow<T, V, L, NV, true>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,    \
+                           static_cast<const T*>(logits), ld, rows, O);                                                      \
+    else                                                                                                                     \
+        hipLaunchKernelGGL((label_scores_narrow<T, V, L, NV, false>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,   \
+                           static_cast<const T*>(logits), ld, rows, O);
+#define BY_WIDTH(T) CBM_LABEL_BY_WIDTH(T, NARROW)
+        CBM_LABEL_BY_TYPE(BY_WIDTH)
+#undef BY_WIDTH
+#undef NARROW
+        return check_launch();
+    }
+#define WIDE(T, TH, NV)                                                                                                     \
+    hipLaunchKernelGGL((label_scores_wide<T, TH, NV>), dim3(rows, s.n), dim3(TH), 0, st, static_cast<const T*>(logits), ld, \
+                       s.cols, workspace, O);
+#define BY_SPLIT(T) CBM_LABEL_BY_SPLIT(T, WIDE)
+#define JOIN(T) \
+    hipLaunchKernelGGL(label_scores_join<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(logits), ld, s.n, workspace, O);
+    CBM_LABEL_BY_TYPE(BY_SPLIT)
+    if (int rc = check_launch()) return rc;
+    if (s.n > 1) { CBM_LABEL_BY_TYPE(JOIN) }
+#undef WIDE
+#undef BY_SPLIT
+#undef JOIN
+    return check_launch();
+}
+
+int grad_rows(const void* logits, void* grad, const Grads& G, int rows, int64_t ld, int64_t ldg, int cols, int dtype, hipStream_t st) {
+    const int classes = G.classes;
+    if (classes <= kNarrowClasses) {
+#define NARROW(T, V, L, NV)                                                                                             \
+    hipLaunchKernelGGL((label_grads_narrow<T, V, L, NV>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,          \
+                       static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, rows, G);
+#define BY_WIDTH(T) CBM_LABEL_BY_WIDTH(T, NARROW)
+        CBM_LABEL_BY_TYPE(BY_WIDTH)
+#undef BY_WIDTH
+#undef NARROW
+        return check_launch();
+    }
+#define WIDE(T)                                                                                                               \
+    hipLaunchKernelGGL(label_grads_wide<T>, dim3(rows, (classes + cols - 1) / cols), dim3(kThreads), 0, st,                   \
+                       static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, cols, G);
+    CBM_LABEL_BY_TYPE(WIDE)
+#undef WIDE
+    return check_launch();
+}
+
+template <typename P>
+P* rows_on(P* p, int64_t n) { return p ? p + n : nullptr; }
+
 }  // namespace
 
 extern "C" {
@@ -587,36 +645,17 @@ int cbm_label_scores(const void* logits, const int64_t* labels, float* logp, flo
     if (rows == 0) return CBM_OK;
     if (!logits || (logp && !labels) || (top > 0 && (!top_logp || !top_index))) return CBM_ERR_NULL;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const Outputs O{labels, logp, entropy, top_logp, top_index, stats, ignore_index, classes, top};
-    if (classes <= kNarrowClasses) {
-#define NARROW(T, V, L, NV)                                                                                                  \
-    if (entropy || top > 0)                                                                                                  \
-        hipLaunchKernelGGL((label_scores_narrow<T, V, L, NV, true>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,    \
-                           static_cast<const T*>(logits), ld, rows, O);                                                      \
-    else                                                                                                                     \
-        hipLaunchKernelGGL((label_scores_narrow<T, V, L, NV, false>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,   \
-                           static_cast<const T*>(logits), ld, rows, O);
-#define BY_WIDTH(T) CBM_LABEL_BY_WIDTH(T, NARROW)
-        CBM_LABEL_BY_TYPE(BY_WIDTH)
-#undef BY_WIDTH
-#undef NARROW
-        return check_launch();
-    }
     const Splits s = splits_of(rows, classes, dtype);
-    if (s.n > 1 && !workspace) return CBM_ERR_NULL;
-#define WIDE(T, TH, NV)                                                                                                     \
-    hipLaunchKernelGGL((label_scores_wide<T, TH, NV>), dim3(rows, s.n), dim3(TH), 0, st, static_cast<const T*>(logits), ld, \
-                       s.cols, workspace, O);
-#define BY_SPLIT(T) CBM_LABEL_BY_SPLIT(T, WIDE)
-#define JOIN(T) \
-    hipLaunchKernelGGL(label_scores_join<T>, dim3(rows), dim3(kThreads), 0, st, static_cast<const T*>(logits), ld, s.n, workspace, O);
-    CBM_LABEL_BY_TYPE(BY_SPLIT)
-    if (int rc = check_launch()) return rc;
-    if (s.n > 1) { CBM_LABEL_BY_TYPE(JOIN) }
-#undef WIDE
-#undef BY_SPLIT
-#undef JOIN
-    return check_launch();
+    if (classes > kNarrowClasses && s.n > 1 && !workspace) return CBM_ERR_NULL;
+    const int most = rows_at_once(classes);
+    for (int64_t r = 0; r < rows; r += most) {
+        const Outputs O{rows_on(labels, r), rows_on(logp, r), rows_on(entropy, r), rows_on(top_logp, r * top), rows_on(top_index, r * top),
+                        rows_on(stats, 2 * r), ignore_index, classes, top};
+        if (int rc = score_rows(static_cast<const char*>(logits) + r * ld * element_bytes(dtype), O, workspace,
+                                static_cast<int>(std::min<int64_t>(most, rows - r)), ld, s, dtype, st))
+            return rc;
+    }
+    return CBM_OK;
 }
 
 int cbm_label_scores_backward(const void* logits, const int64_t* labels, const float* stats, const float* entropy, const int64_t* top_index,
@@ -628,27 +667,19 @@ int cbm_label_scores_backward(const void* logits, const int64_t* labels, const f
     if (!logits || !stats || !grad || (g_logp && !labels) || (g_entropy && !entropy) || (g_top && (!top_index || top < 1)))
         return CBM_ERR_NULL;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const Grads G{labels, stats, entropy, top_index, g_logp, g_entropy, g_top, ignore_index, classes, top};
-    if (classes <= kNarrowClasses) {
-#define NARROW(T, V, L, NV)                                                                                             \
-    hipLaunchKernelGGL((label_grads_narrow<T, V, L, NV>), dim3(narrow_blocks(rows, L)), dim3(kThreads), 0, st,          \
-                       static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, rows, G);
-#define BY_WIDTH(T) CBM_LABEL_BY_WIDTH(T, NARROW)
-        CBM_LABEL_BY_TYPE(BY_WIDTH)
-#undef BY_WIDTH
-#undef NARROW
-        return check_launch();
-    }
     // a workgroup per share of a row: kGradVectors vectors a thread, fewer where rows are few
-    const int V = 16 / element_bytes(dtype);
+    const int V = 16 / element_bytes(dtype), most = rows_at_once(classes);
     int cols = kThreads * kGradVectors * V;
     while (cols > kThreads * V && static_cast<int64_t>(rows) * ((classes + cols - 1) / cols) < 1024) cols >>= 1;
-#define WIDE(T)                                                                                                               \
-    hipLaunchKernelGGL(label_grads_wide<T>, dim3(rows, (classes + cols - 1) / cols), dim3(kThreads), 0, st,                   \
-                       static_cast<const T*>(logits), static_cast<T*>(grad), ld, ldg, cols, G);
-    CBM_LABEL_BY_TYPE(WIDE)
-#undef WIDE
-    return check_launch();
+    for (int64_t r = 0; r < rows; r += most) {
+        const Grads G{rows_on(labels, r), rows_on(stats, 2 * r), rows_on(entropy, r), rows_on(top_index, r * top), rows_on(g_logp, r),
+                      rows_on(g_entropy, r), rows_on(g_top, r * top), ignore_index, classes, top};
+        if (int rc = grad_rows(static_cast<const char*>(logits) + r * ld * element_bytes(dtype),
+                               static_cast<char*>(grad) + r * ldg * element_bytes(dtype), G,
+                               static_cast<int>(std::min<int64_t>(most, rows - r)), ld, ldg, cols, dtype, st))
+            return rc;
+    }
+    return CBM_OK;
 }
 
 }  // extern "C"

@@ -887,6 +887,8 @@ Plan plan_of(const cbm_norm_batch* B, int C, int groups, int dtype, bool backwar
     return P;
 }
 
+static_assert(sizeof(cbm_norm_batch) == 56, "the layout that bindings mirror");
+
 Rows rows_of(const cbm_norm_batch* B) {
     Rows R{};
     R.pieces = reinterpret_cast<const int4*>(B->pieces);
@@ -905,16 +907,18 @@ int check_batch(const cbm_norm_batch* B, int C, int groups, int dtype, int act) 
     if (dtype < CBM_DTYPE_F32 || dtype > CBM_DTYPE_F16 || act < CBM_ACT_NONE || act > CBM_ACT_SILU) return CBM_ERR_SHAPE;
     if (C < 1 || C > (1 << 16) || groups < 1 || C % groups) return CBM_ERR_SHAPE;
     if (B->samples < 0 || B->rows < 0 || B->max_len < 0 || B->max_len > B->rows) return CBM_ERR_SHAPE;
-    if (static_cast<int64_t>(B->samples) * groups > (1 << 30)) return CBM_ERR_SHAPE;
+    if (B->samples > CBM_NORM_MAX_GRAPHS || static_cast<int64_t>(B->samples) * groups > CBM_NORM_MAX_PAIRS) return CBM_ERR_SHAPE;
     if (!B->ptr && static_cast<int64_t>(B->samples) * B->max_len != B->rows) return CBM_ERR_SHAPE;
     if (B->ptr && B->rows > 0 && (!B->pieces || !B->piece_ptr || B->n_pieces < 1)) return CBM_ERR_NULL;
     if (B->rows > 0 && B->piece_rows < 1) return CBM_ERR_SHAPE;
     return CBM_OK;
 }
 
-// Threads that join the pieces of a (sample, group), by its number of partial results.
-int join_threads(int pieces, int D, int samples) {
+// Threads that join the pieces of a (sample, group), by its number of partial results; a grid holds fewer than 2^32 threads
+// along one dimension (the limits on graphs and pairs keep the others below that).
+int join_threads(int pieces, int D, int samples, int groups) {
     const int64_t items = static_cast<int64_t>(pieces) * D / samples;
+    if (static_cast<int64_t>(samples) * groups > (1 << 21)) return kWave;
     return items >= 2048 ? kMaxThreads : items >= 256 ? 256 : kWave;
 }
 
@@ -990,7 +994,7 @@ int cbm_group_norm_forward(const cbm_norm_batch* B, const void* X, void* Y, cons
                        static_cast<T*>(Y), weight, bias, m, r, R, S)
     CBM_NORM_BY_TYPE(8, STATS)
     if (int rc = check_launch()) return rc;
-    hipLaunchKernelGGL(norm_join_stats, dim3(static_cast<unsigned>(pairs)), dim3(join_threads(np, S.D, B->samples)), 0, st,
+    hipLaunchKernelGGL(norm_join_stats, dim3(static_cast<unsigned>(pairs)), dim3(join_threads(np, S.D, B->samples, groups)), 0, st,
                        part, m, r, R, S);
     if (int rc = check_launch()) return rc;
     CBM_NORM_BY_TYPE(8, APPLY)
@@ -1049,7 +1053,7 @@ int cbm_group_norm_backward(const cbm_norm_batch* B, const void* X, const void* 
     CBM_NORM_BY_TYPE(8, SUMS)
     if (int rc = check_launch()) return rc;
     // both joins in one launch, unless the pairs are many and small
-    const int threads = join_threads(np, S.D, B->samples);
+    const int threads = join_threads(np, S.D, B->samples, groups);
     const bool apart = params && threads < kMaxThreads;
     hipLaunchKernelGGL(norm_join_grads, dim3(pairs + (params && !apart ? channel_blocks : 0)), dim3(threads), 0, st, part, weight, c1, c2,
                        dweight, dbias, pairs, np, R, S);

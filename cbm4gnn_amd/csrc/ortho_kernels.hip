@@ -610,7 +610,7 @@ __global__ __launch_bounds__(kWave* kSmallWaves) void ortho_product_small(const 
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-constexpr int64_t kMaxTiles = 1LL << 30;
+constexpr int64_t kMaxTiles = 1LL << 25;   // of 32 x 32 in a turn: far beyond memory, and every grid stays below 2^32 threads
 
 int padded(int v, int unit) { return (v + unit - 1) / unit * unit; }
 
@@ -675,6 +675,7 @@ int64_t lay_out(const cbm_ortho_item* items, int n, Items& L, Choice& choice) {
 }
 
 constexpr int64_t kNormBytes = static_cast<int64_t>(kMaxItems) * kNormBlocks * sizeof(double);
+static_assert(sizeof(cbm_ortho_item) == 72, "the layout that bindings mirror");
 constexpr int64_t kListBytes = 4096;
 static_assert(sizeof(Items) <= kListBytes, "the list");
 

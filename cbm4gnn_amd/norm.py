@@ -184,8 +184,9 @@ def group_norm(x, groups, weight=None, bias=None, *, graphs=None, eps=1e-5, acti
     _check_channel(bias, "bias", ch, x.device)
     m = rows_view(x, "x")
     samples = graphs.n_graphs if graphs is not None else 1 if x.dim() == 2 else x.size(0)
-    if samples * groups > 1 << 30:
-        raise ValueError("graphs times groups: at most 2^30")
+    if samples > _lib.CBM_NORM_MAX_GRAPHS or samples * groups > _lib.CBM_NORM_MAX_PAIRS:
+        raise ValueError(f"{samples} graphs of {groups} groups: at most {_lib.CBM_NORM_MAX_GRAPHS} graphs, and "
+                         f"{_lib.CBM_NORM_MAX_PAIRS} graphs times groups")
     if graphs is None:
         check_int32(x.numel() // ch, "rows of x")
     _require_gpu()

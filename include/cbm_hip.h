@@ -624,7 +624,8 @@ enum { CBM_ACT_NONE = 0, CBM_ACT_RELU = 1, CBM_ACT_SILU = 2 };
  * into pieces of at most piece_rows, no piece across two graphs: pieces (device, n_pieces times {graph, first
  * row, rows, 0}, by graph and row) and piece_ptr (device, samples + 1: first piece of each graph).  order
  * (device, samples, may be NULL): the graphs in the order they are begun in, longest first.  The kernels index
- * with these arrays as they are. */
+ * with these arrays as they are.  At most CBM_NORM_MAX_GRAPHS graphs, and CBM_NORM_MAX_PAIRS graphs times groups. */
+enum { CBM_NORM_MAX_GRAPHS = 1 << 21, CBM_NORM_MAX_PAIRS = 1 << 25 };
 typedef struct cbm_norm_batch {
     int32_t samples, max_len, rows, piece_rows, n_pieces, reserved;
     const int32_t* ptr;

@@ -8,7 +8,7 @@ import sys
 import pytest
 import torch
 
-from cbm4gnn_amd.labels import label_log_probs
+from cbm4gnn_amd.labels import LabelScores, label_log_probs
 
 U = 2.0 ** -24
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -344,6 +344,39 @@ def test_captured_graphs_replay(gpu, rows, classes):
             torch.cuda.synchronize()
             for p, q, r in zip(out, want, eager):
                 assert torch.equal(p, q) and torch.equal(r, q), turn
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,dtype", [((1 << 25) + 5, 3, F32), ((1 << 21) + 3, 1100, BF16)])
+def test_more_rows_than_one_launch(gpu, rows, classes, dtype):
+    say("rows", rows, classes, dtype)
+    g = torch.Generator(device=gpu).manual_seed(1)
+    z = torch.randn((rows, classes), generator=g, device=gpu, dtype=dtype).requires_grad_()
+    y = torch.randint(0, classes, (rows,), generator=g, device=gpu)
+    y[::7] = IGNORE
+    g_logp = torch.randn(rows, generator=g, device=gpu)
+    r = label_log_probs(z, y, entropy=True, top=2)
+    grad, = torch.autograd.grad(r.logp, z, g_logp)
+    edge = 1 << (25 if classes < 1024 else 21)
+    at = torch.cat([torch.arange(0, 200), torch.arange(edge - 100, rows)]).to(gpu)
+    # a row's scores and gradient depend on nothing but the row: the same bits as those of a call of its own
+    part = z.detach()[at].requires_grad_()
+    q = label_log_probs(part, y[at], entropy=True, top=2)
+    alone, = torch.autograd.grad(q.logp, part, g_logp[at])
+    for name in r._fields:
+        assert torch.equal(getattr(r, name).detach()[at], getattr(q, name).detach()), name
+    assert torch.equal(grad[at], alone)
+    compare(LabelScores(*(t.detach().cpu() for t in q)), part.detach().cpu(), y[at].cpu(), 2, "edge rows")
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused(gpu):
+    z, y = torch.randn((40, 8), device=gpu, requires_grad=True), torch.arange(40, device=gpu) % 8
+    grad, = torch.autograd.grad(label_log_probs(z, y).logp.sum(), z, create_graph=True)
+    plain, = torch.autograd.grad(label_log_probs(z, y).logp.sum(), z)
+    assert torch.equal(grad, plain)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
 
 
 def test_refusals():

@@ -6,12 +6,14 @@ Tolerances count roundings.  With u = 2^-24 (half a step of fp32), a statistic o
 no sum is longer than the graph's rows, so n u (sum of magnitudes) bounds its error, and 2^-21 covers the dozen
 roundings of one element (subtract, scale, shift, exp with its argument, quotient, products).  A result in fewer bits
 adds half a step of its type, ``finfo.eps / 2`` relative."""
+import ctypes as C
 import sys
 
 import numpy as np
 import pytest
 import torch
 
+from cbm4gnn_amd import _lib
 from cbm4gnn_amd.norm import GraphBatch, GroupNorm, group_norm
 
 U = 2.0 ** -24
@@ -342,6 +344,54 @@ def test_captured_graphs_replay(gpu, rows, graphs):
             torch.cuda.synchronize()
             for p, q, r in zip(out, want, eager):
                 assert torch.equal(p, q) and torch.equal(r, q), turn
+
+
+@pytest.mark.gpu
+def test_many_short_graphs_behind_a_long_one(gpu):
+    """More graphs times groups than a join of 1024 threads each may have in one launch.  Whole numbers in dy: their
+    sums are exact in any order."""
+    short, ch, long = 300_000, 8, 20_000
+    rows = long + 3 * short
+    say("many pairs", rows, short)
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn((rows, ch), generator=g) + torch.randn(ch, generator=g)
+    dy = torch.randint(-3, 4, (rows, ch), generator=g).float()
+    w, b = 1 + 0.1 * torch.randn(ch, generator=g), 0.1 * torch.randn(ch, generator=g)
+    ptr = np.concatenate([[0], long + 3 * np.arange(short + 1)])
+    leaves = [t.to(gpu).requires_grad_() for t in (x, w, b)]
+    y = group_norm(leaves[0], ch, leaves[1], leaves[2], graphs=GraphBatch(ptr))
+    dx, _, db = torch.autograd.grad(y, leaves, dy.to(gpu))
+    assert torch.equal(db.cpu(), dy.sum(0))
+    picks = [0, 1, 2, short] + np.random.default_rng(0).integers(1, short, 100).tolist()
+    at = torch.cat([torch.arange(ptr[p], ptr[p + 1]) for p in picks])
+    sub = np.concatenate([[0], np.cumsum([ptr[p + 1] - ptr[p] for p in picks])]).tolist()
+    ry, rdx, _, _, ey, edx, _, _ = reference(x[at], ch, w, b, sub, 1e-5, "none", dy[at])
+    close(y.detach().cpu()[at], ry, ey, F32, "y")
+    close(dx.cpu()[at], rdx, edx, F32, "dx")
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused(gpu):
+    x = torch.randn((40, 8), device=gpu, requires_grad=True)
+    dx, = torch.autograd.grad(group_norm(x, 2, activation="silu").sum(), x, create_graph=True)
+    plain, = torch.autograd.grad(group_norm(x, 2, activation="silu").sum(), x)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+def test_struct_layout():
+    assert C.sizeof(_lib.CbmNormBatch) == 56 and _lib.CbmNormBatch.ptr.offset == 24
+    assert C.sizeof(_lib.CbmOrthoItem) == 72 and _lib.CbmOrthoItem.ld_src.offset == 40
+
+
+def test_too_many_graphs():
+    with pytest.raises(ValueError, match="at most"):
+        group_norm(torch.empty(((1 << 21) + 1, 1, 2)), 1)
+    with pytest.raises(ValueError, match="at most"):
+        group_norm(torch.empty((1 << 20, 1, 33)), 33)
+    with pytest.raises(ValueError, match="at most"):
+        group_norm(torch.empty((0, 2)), 1, graphs=GraphBatch(np.zeros((1 << 21) + 2, dtype=np.int64)))
 
 
 def test_refusals():
