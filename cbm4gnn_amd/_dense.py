@@ -1,10 +1,7 @@
 """What the dense operators (``norm``, ``labels``, ``optim``) share: element types, layout checks, launches."""
 from __future__ import annotations
 
-import functools
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from .cbm import _require_gpu, _stream  # noqa: F401  (the streams and the no-GPU error are the multiply's)
 
@@ -45,28 +42,8 @@ def rows_view(t, name):
     return m
 
 
-def grad_rows(g, rows, width):
-    """An incoming gradient as [rows, width] with unit column stride; copied where autograd hands over another
-    layout (an expanded scalar, a transpose)."""
-    if g.dim() != 2:
-        g = g.reshape(rows, width)
-    if (width > 1 and g.stride(1) != 1) or (rows > 1 and g.stride(0) < width):
-        g = g.contiguous()
-    return g
-
-
 def ld(t):
     return t.stride(0) if t.size(0) > 1 else max(t.size(1), 1)
-
-
-def once(backward):
-    """``once_differentiable`` where a graph of the gradient is asked for; its 10 us are spent nowhere else."""
-    guarded = once_differentiable(backward)
-
-    @functools.wraps(backward)
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
 
 
 def ptr(t):

@@ -1,4 +1,5 @@
-"""ctypes bindings of the two C-ABI libraries declared in ``include/cbm_hip.h``.
+"""ctypes bindings of the two C-ABI libraries declared in ``include/cbm_hip.h``, and the extension module that puts
+the dense operators under torch's autograd.
 
 The libraries are loaded from ``cbm4gnn_amd/lib`` (built in-tree by ``cbm4gnn_amd.build``).
 There is no fallback of any kind: a missing library raises ``CbmLibraryError`` and a non-zero
@@ -7,9 +8,10 @@ status from a call raises ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 
-from .build import HIP_LIB, HOST_LIB
+from .build import AUTOGRAD_LIB, HIP_LIB, HOST_LIB
 
 CBM_OK = 0
 CBM_PROP_SCALE_ROOTS = 1
@@ -200,6 +202,7 @@ HIP_SYMBOLS = {
 
 _host = None
 _hip = None
+_autograd = None
 
 
 def _load(path: str, symbols: dict, what: str):
@@ -233,6 +236,24 @@ def hip_lib():
     if _hip is None:
         _hip = _load(HIP_LIB, HIP_SYMBOLS, "HIP kernel")
     return _hip
+
+
+def autograd_lib():
+    global _autograd
+    if _autograd is None:
+        import torch  # noqa: F401  (the module is linked to its libraries)
+        hip_lib()                                           # the same error where that is missing
+        if not os.path.exists(AUTOGRAD_LIB):
+            raise CbmLibraryError(f"autograd library not found at {AUTOGRAD_LIB}; build it with `python -m cbm4gnn_amd.build` "
+                                  "(there is no fallback)")
+        spec = importlib.util.spec_from_file_location("cbm_autograd", AUTOGRAD_LIB)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:                            # e.g. built against another torch
+            raise CbmLibraryError(f"cannot load {AUTOGRAD_LIB}: {e}") from e
+        _autograd = module
+    return _autograd
 
 
 def check(status: int, where: str):

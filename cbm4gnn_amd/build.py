@@ -1,7 +1,8 @@
-"""Build the two shared libraries of the package in-tree.
+"""Build the shared libraries of the package in-tree.
 
-    libcbm_hip.so   hipcc, gfx950 only: the HIP kernels and their C-ABI launchers
-    libcbm_host.so  g++ / OpenMP: the host-side format builder
+    libcbm_hip.so    hipcc, gfx950 only: the HIP kernels and their C-ABI launchers
+    libcbm_host.so   g++ / OpenMP: the host-side format builder
+    cbm_autograd.so  g++ against torch: the dense operators' autograd nodes, over libcbm_hip.so
 
 Run ``python -m cbm4gnn_amd.build`` (no GPU needed: hipcc cross-compiles).  The reference builds
 its extension with cmake + setuptools against MKL and arbok (``cbm/setup.py:15-47``); none of
@@ -20,6 +21,7 @@ SRC_DIR = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 HIP_LIB = os.path.join(LIB_DIR, "libcbm_hip.so")
 HOST_LIB = os.path.join(LIB_DIR, "libcbm_host.so")
+AUTOGRAD_LIB = os.path.join(LIB_DIR, "cbm_autograd.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -63,8 +65,32 @@ def build_host(verbose: bool = False) -> str:
     return HOST_LIB
 
 
+def build_autograd(verbose: bool = False) -> str:
+    """After ``build_hip``, whose library it is linked to."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    include, libs = os.path.join(root, "include"), os.path.join(root, "lib")
+    rocm = os.path.dirname(os.path.dirname(HIPCC))
+    out = _run(["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                *(f"-isystem{d}" for d in (include, os.path.join(include, "torch", "csrc", "api", "include"),
+                                           sysconfig.get_paths()["include"], os.path.join(rocm, "include"))),
+                "-o", AUTOGRAD_LIB, os.path.join(SRC_DIR, "dense_autograd.cpp"),
+                f"-L{LIB_DIR}", "-l:libcbm_hip.so", "-Wl,-rpath,$ORIGIN",
+                f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"])
+    if verbose and out.strip():
+        print(out)
+    return AUTOGRAD_LIB
+
+
 def build_all(verbose: bool = False):
-    return build_hip(verbose), build_host(verbose)
+    """Side by side, but for what is linked to another."""
+    with ThreadPoolExecutor(1) as pool:
+        host = pool.submit(build_host, verbose)
+        return build_hip(verbose), build_autograd(verbose), host.result()
 
 
 if __name__ == "__main__":

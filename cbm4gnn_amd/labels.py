@@ -11,13 +11,12 @@ Calls on CPU tensors are staged through the GPU, as the multiply's are.
 """
 from __future__ import annotations
 
-import functools
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from ._dense import DTYPES, _require_gpu, _stream, check_dtype, check_int32, ld, on_device, once, ptr, rows_view
+from ._dense import _require_gpu, check_dtype, check_int32, rows_view
 
 __all__ = ["LabelScores", "label_log_probs"]
 
@@ -29,57 +28,6 @@ class LabelScores(NamedTuple):
     entropy: Optional[torch.Tensor]
     top_logp: Optional[torch.Tensor]
     top_index: Optional[torch.Tensor]
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_floats(rows, classes, top, dtype):
-    return _lib.hip_lib().cbm_label_scores_workspace_floats(rows, classes, top, dtype)
-
-
-def _forward(z, labels, entropy, top, ignore_index, keep):
-    rows, classes = z.shape
-    dev, dt, f32 = z.device, DTYPES[z.dtype], torch.float32
-    logp = torch.empty(rows, dtype=f32, device=dev) if labels is not None else None
-    ent = torch.empty(rows, dtype=f32, device=dev) if entropy else None
-    top_logp = torch.empty((rows, top), dtype=f32, device=dev) if top else None
-    top_index = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty((rows, 2), dtype=f32, device=dev) if keep else None
-    floats = _workspace_floats(rows, classes, top, dt)
-    ws = torch.empty(floats, dtype=f32, device=dev) if floats else None
-    with on_device(dev):
-        rc = _lib.hip_lib().cbm_label_scores(ptr(z), ptr(labels), ptr(logp), ptr(ent), ptr(top_logp), ptr(top_index), ptr(stats), ptr(ws),
-                                             rows, classes, top, ld(z), ignore_index, dt, _stream(dev))
-    if rc:
-        _lib.check(rc, "cbm_label_scores")
-    return logp, ent, top_logp, top_index, stats
-
-
-class _LabelScores(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, labels, entropy, top, ignore_index):
-        logp, ent, top_logp, top_index, stats = _forward(z, labels, entropy, top, ignore_index, True)
-        ctx.save_for_backward(z, labels, stats, ent, top_index)
-        ctx.top, ctx.ignore_index = top, ignore_index
-        ctx.set_materialize_grads(False)
-        if top_index is not None:
-            ctx.mark_non_differentiable(top_index)
-        return logp, ent, top_logp, top_index
-
-    @staticmethod
-    @once
-    def backward(ctx, g_logp, g_ent, g_top, _):
-        z, labels, stats, ent, top_index = ctx.saved_tensors
-        rows, classes = z.shape
-        dev, dt = z.device, DTYPES[z.dtype]
-        flat = [g if g is None or g.is_contiguous() else g.contiguous() for g in (g_logp, g_ent, g_top)]
-        grad = torch.empty((rows, classes), dtype=z.dtype, device=dev)
-        with on_device(dev):
-            rc = _lib.hip_lib().cbm_label_scores_backward(
-                ptr(z), ptr(labels), ptr(stats), ptr(ent), ptr(top_index), ptr(flat[0]), ptr(flat[1]), ptr(flat[2]), ptr(grad), rows,
-                classes, ctx.top, ld(z), classes, ctx.ignore_index, dt, _stream(dev))
-        if rc:
-            _lib.check(rc, "cbm_label_scores_backward")
-        return grad, None, None, None, None
 
 
 def label_log_probs(logits, labels=None, *, entropy=False, top=0, ignore_index=-100) -> LabelScores:
@@ -124,10 +72,7 @@ def label_log_probs(logits, labels=None, *, entropy=False, top=0, ignore_index=-
     if labels is not None:
         if labels.dtype != torch.int64 or labels.dim() != 1 or not labels.is_contiguous():
             labels = labels.reshape(rows).to(torch.int64).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        parts = _LabelScores.apply(z, labels, bool(entropy), top, ignore_index)
-    else:
-        parts = _forward(z, labels, bool(entropy), top, ignore_index, False)[:4]
+    parts = _lib.autograd_lib().label_scores(z, labels, bool(entropy), top, ignore_index)
     if logits.dim() != 2:
         parts = tuple(None if t is None else t.reshape((*lead, *t.shape[1:])) for t in parts)
     return LabelScores(*parts)

@@ -12,7 +12,6 @@ torch's current stream and return.  Calls on CPU tensors are staged through the 
 """
 from __future__ import annotations
 
-import ctypes as C
 import functools
 
 import numpy as np
@@ -20,7 +19,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._dense import DTYPES, _require_gpu, _stream, check_dtype, check_int32, grad_rows, ld, on_device, once, ptr, rows_view
+from ._dense import _require_gpu, _stream, check_dtype, check_int32, rows_view
 
 __all__ = ["GraphBatch", "group_norm", "GroupNorm"]
 
@@ -36,9 +35,9 @@ def _piece_rows(rows):
 
 @functools.lru_cache(maxsize=64)
 def _equal_batch(samples, length):
-    """``cbm_norm_batch`` of ``samples`` graphs of ``length`` nodes each."""
+    """The rows of ``samples`` graphs of ``length`` nodes each."""
     rows = samples * length
-    return _lib.CbmNormBatch(samples=samples, max_len=length, rows=rows, piece_rows=_piece_rows(rows))
+    return _lib.autograd_lib().NormBatch(samples, length, rows, _piece_rows(rows), 0, [])
 
 
 class GraphBatch:
@@ -80,64 +79,14 @@ class GraphBatch:
         held = self._on.get(device)
         if held is None:
             arrays = [torch.from_numpy(a).to(device) for a in (self._ptr, self._pieces, self._piece_ptr, self._order)]
-            st = _lib.CbmNormBatch(samples=self.n_graphs, max_len=self.max_nodes, rows=self.n_nodes, piece_rows=self._rows,
-                                   n_pieces=len(self._pieces), ptr=ptr(arrays[0]), pieces=ptr(arrays[1]), piece_ptr=ptr(arrays[2]),
-                                   order=ptr(arrays[3]))
-            st.arrays = arrays                              # whoever holds the struct (a backward to come) holds what it points at
+            # whoever holds the struct (a backward to come) holds the arrays
+            st = _lib.autograd_lib().NormBatch(self.n_graphs, self.max_nodes, self.n_nodes, self._rows, len(self._pieces), arrays)
             held = self._on[device] = (st, _stream(device).value)
         st, home = held
         if _stream(device).value != home:                   # not to be reused for others before this stream is done with them
             for a in st.arrays:
                 a.record_stream(torch.cuda.current_stream(device))
         return st
-
-
-def _forward(x, m, weight, bias, batch, groups, eps, act, keep):
-    ch, dev, dt, f32 = m.size(1), x.device, DTYPES[x.dtype], torch.float32
-    lib, b = _lib.hip_lib(), C.byref(batch)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean = rstd = None
-    if keep:
-        mean = torch.empty((batch.samples, groups), dtype=f32, device=dev)
-        rstd = torch.empty((batch.samples, groups), dtype=f32, device=dev)
-    floats = lib.cbm_group_norm_workspace_floats(b, ch, groups, dt, 0)
-    ws = torch.empty(floats, dtype=f32, device=dev) if floats else None
-    with on_device(dev):
-        rc = lib.cbm_group_norm_forward(b, ptr(m), ptr(y), ptr(weight), ptr(bias), ptr(mean), ptr(rstd), ptr(ws), ch, groups,
-                                        ld(m), ch, eps, act, dt, _stream(dev))
-    if rc:
-        _lib.check(rc, "cbm_group_norm_forward")
-    return y, mean, rstd
-
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, batch, groups, eps, act):
-        y, mean, rstd = _forward(x, rows_view(x, "x"), weight, bias, batch, groups, eps, act, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.batch, ctx.groups, ctx.act = batch, groups, act
-        return y
-
-    @staticmethod
-    @once
-    def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        m = rows_view(x, "x")
-        rows, ch = m.shape
-        g = grad_rows(dy, rows, ch)
-        need, dev, dt, f32 = ctx.needs_input_grad, x.device, DTYPES[x.dtype], torch.float32
-        lib, b = _lib.hip_lib(), C.byref(ctx.batch)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-        dw = torch.empty(ch, dtype=f32, device=dev) if need[1] else None
-        db = torch.empty(ch, dtype=f32, device=dev) if need[2] else None
-        floats = lib.cbm_group_norm_workspace_floats(b, ch, ctx.groups, dt, 1)
-        ws = torch.empty(floats, dtype=f32, device=dev) if floats else None
-        with on_device(dev):
-            rc = lib.cbm_group_norm_backward(b, ptr(m), ptr(g), ptr(dx), ptr(weight), ptr(bias), ptr(mean), ptr(rstd), ptr(dw), ptr(db),
-                                             ptr(ws), ch, ctx.groups, ld(m), ld(g), ch, ctx.act, dt, _stream(dev))
-        if rc:
-            _lib.check(rc, "cbm_group_norm_backward")
-        return dx, dw, db, None, None, None, None
 
 
 def _check_channel(t, name, ch, device):
@@ -182,7 +131,7 @@ def group_norm(x, groups, weight=None, bias=None, *, graphs=None, eps=1e-5, acti
             raise ValueError(f"x has {x.size(0)} rows, the batch has {graphs.n_nodes} nodes")
     _check_channel(weight, "weight", ch, x.device)
     _check_channel(bias, "bias", ch, x.device)
-    m = rows_view(x, "x")
+    rows_view(x, "x")
     samples = graphs.n_graphs if graphs is not None else 1 if x.dim() == 2 else x.size(0)
     if samples > _lib.CBM_NORM_MAX_GRAPHS or samples * groups > _lib.CBM_NORM_MAX_PAIRS:
         raise ValueError(f"{samples} graphs of {groups} groups: at most {_lib.CBM_NORM_MAX_GRAPHS} graphs, and "
@@ -195,10 +144,7 @@ def group_norm(x, groups, weight=None, bias=None, *, graphs=None, eps=1e-5, acti
         return group_norm(staged[0], groups, *staged[1:], graphs=graphs, eps=eps, activation=activation).to(x.device)
     batch = graphs._struct(x.device) if graphs is not None else _equal_batch(samples, x.numel() // ch // samples if samples else 0)
     act = _lib.CBM_ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
-        return _GroupNorm.apply(x, weight, bias, batch, groups, eps, act)
-    return _forward(x, m, weight, bias, batch, groups, eps, act, False)[0]
+    return _lib.autograd_lib().group_norm(x, weight, bias, batch, groups, eps, act)
 
 
 class GroupNorm(nn.Module):

@@ -385,6 +385,13 @@ def test_struct_layout():
     assert C.sizeof(_lib.CbmOrthoItem) == 72 and _lib.CbmOrthoItem.ld_src.offset == 40
 
 
+def test_a_missing_autograd_library_fails_loudly(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_autograd", None)
+    monkeypatch.setattr(_lib, "AUTOGRAD_LIB", str(tmp_path / "nope.so"))
+    with pytest.raises(_lib.CbmLibraryError):
+        _lib.autograd_lib()
+
+
 def test_too_many_graphs():
     with pytest.raises(ValueError, match="at most"):
         group_norm(torch.empty(((1 << 21) + 1, 1, 2)), 1)
