@@ -21,7 +21,7 @@
 // Measured (one MI355X, kernel times):
 //   one graph of 232 965 nodes, 128 channels, fp32, SiLU, in pieces: forward 33 + 7 + 39 us, backward 44 + 7 + 55 us; the
 //   passes move 3.6, 6.1, 5.4 and 6.5 TB/s against 5.1 of a 2 GiB copy (what the last-level cache holds comes on top)
-//   2 000 graphs, 100 000 nodes, 256 channels, bf16, SiLU, in one launch: forward 38, backward 61 + 6 us; half of it is
+//   2 000 graphs, 100 000 nodes, 256 channels, bf16, SiLU, in one launch: forward 38 to 41, backward 59 to 62 + 6 us; half of it is
 //   arithmetic (28 and 53 vector instructions a value), the rest latency of a graph at a time
 //   512 nodes, 64 channels, fp32, ReLU: forward 6.6 us
 //
