@@ -59,7 +59,8 @@ def _workspace(lib, items, n, device):
 def orthogonalise(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
     """``steps`` Newton-Schulz steps on ``g`` / (|g| + eps): [rows, cols], or [..., rows, cols] for a batch of
     matrices.  float32, bfloat16 or float16; returns a contiguous tensor of its shape and type, outside
-    autograd.  Matrices need unit stride along columns.  Zeros give zeros."""
+    autograd.  Matrices need unit stride along columns.  Zeros give zeros.  Products keep operands as fp16 pairs:
+    coefficients under which values grow beyond 65 504 give infinities."""
     check_dtype(g, "g")
     steps, abc, eps = _check_steps(steps, coefficients, eps)
     if g.dim() < 2:

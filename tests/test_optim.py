@@ -130,6 +130,18 @@ def test_sizes_of_values_and_special_ones(gpu):
     assert torch.equal(orthogonalise(g), orthogonalise(g.to(gpu)).cpu())
 
 
+@pytest.mark.gpu
+def test_norms_outside_fp32(gpu):
+    """Powers of two come out of X = G / |G| exactly, so the bits are those of the unscaled matrix."""
+    say("ortho scales")
+    g = torch.randint(-7, 8, (64, 80), generator=torch.Generator().manual_seed(9)).float()
+    want = orthogonalise(g.to(gpu), eps=0.0)
+    for power in (120, 124, -100, -145):                    # |G| = 2^8.2: beyond fp32 at 120; subnormal elements at -145
+        scaled = torch.ldexp(g.double(), torch.tensor(power)).float()
+        assert torch.isfinite(scaled).all() and torch.equal(scaled.double(), g.double() * 2.0 ** power)
+        assert torch.equal(orthogonalise(scaled.to(gpu), eps=0.0), want), power
+
+
 def muon_reference(w, g, m, lr, mu, decay, nesterov):
     m = mu * m.double() + g.double()
     o, err = exact(g.double() + mu * m if nesterov else m)
