@@ -73,6 +73,9 @@ class GraphBatch:
             _require_gpu()
             self._struct(torch.device(device))
 
+    def __getstate__(self):
+        return {**self.__dict__, "_on": {}}                 # a copy makes its own device arrays
+
     def _struct(self, device):
         if device.index is None:
             device = torch.device(device.type, torch.cuda.current_device())
