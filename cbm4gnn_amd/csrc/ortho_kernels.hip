@@ -115,6 +115,12 @@ __device__ __forceinline__ void split4(float v, half4& hi, half4& lo, int e) {
     hi[e] = a;
     lo[e] = b;
 }
+// Stores of planes go through the XCD's L2 at once (agent scope): the next launch reads them from the other XCDs, and what is
+// dirty in the L2 when a launch ends is written back then, with nothing left to overlap it.  8 x 512 x 1024, the whole call:
+// 287 us for 310; stores that also skip the last-level cache (non-temporal): 327.
+__device__ __forceinline__ void put(_Float16* to, half4 v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 __device__ __forceinline__ float whole(_Float16 hi, _Float16 lo) {
     return __builtin_fmaf(static_cast<float>(lo), 1.f / kLo, static_cast<float>(hi));
 }
@@ -220,15 +226,15 @@ __global__ __launch_bounds__(256) void ortho_split(const Items* __restrict__ lis
 #pragma unroll
             for (int e = 0; e < 4; ++e) split4(tile[u][f + e], hi, lo, e);
             const int64_t at = static_cast<int64_t>(i0 + u) * I.ll + j0 + f;
-            *reinterpret_cast<half4*>(P.x + at) = hi;
-            *reinterpret_cast<half4*>(P.x + P.nx + at) = lo;
+            put(P.x + at, hi);
+            put(P.x + P.nx + at, lo);
         }
         if (j0 + u < I.lp && i0 + f < I.sp) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) split4(tile[f + e][u], hi, lo, e);
             const int64_t to = static_cast<int64_t>(j0 + u) * I.ls + i0 + f;
-            *reinterpret_cast<half4*>(P.xt[0] + to) = hi;
-            *reinterpret_cast<half4*>(P.xt[0] + P.nt + to) = lo;
+            put(P.xt[0] + to, hi);
+            put(P.xt[0] + P.nt + to, lo);
         }
     }
 }
@@ -278,20 +284,27 @@ __device__ __forceinline__ Operands operands_of(const Item& I, const Planes& P, 
     return O;
 }
 
-// What a product leaves for four rows i .. i + 3 of column j, given their sums in v: the new values, which go to X^T, A or
-// B (four halves along memory) and come back as words {hi, lo} for the row order, or as they are for the result.
+// What a product adds to in four rows i .. i + 3 of column j: A (poly) or X^T (apply).
+struct Old { half4 hi, lo; };
 template <Kind KIND>
-__device__ __forceinline__ void finish_column(const Item& I, const Planes& P, const Poly& C, int turn, int i, int j, float (&v)[4],
-                                              uint32_t (&w)[4]) {
+__device__ __forceinline__ Old old_values(const Item& I, const Planes& P, int turn, int i, int j) {
+    const int64_t at = static_cast<int64_t>(j) * I.ls + i;
+    if constexpr (KIND == kPoly) return {*reinterpret_cast<const half4*>(P.a + at), *reinterpret_cast<const half4*>(P.a + P.na + at)};
+    else if constexpr (KIND != kGram)
+        return {*reinterpret_cast<const half4*>(P.xt[turn] + at), *reinterpret_cast<const half4*>(P.xt[turn] + P.nt + at)};
+    else return {};
+}
+
+// What a product leaves there, given their sums in v: the new values, which go to X^T, A or B (four halves along memory) and
+// come back as words {hi, lo} for the row order, or as they are for the result.
+template <Kind KIND>
+__device__ __forceinline__ void finish_column(const Item& I, const Planes& P, const Poly& C, int turn, int i, int j, const Old& old,
+                                              float (&v)[4], uint32_t (&w)[4]) {
     const int64_t to = static_cast<int64_t>(j) * I.ls + i;
-    if constexpr (KIND == kPoly) {
-        const half4 h = *reinterpret_cast<const half4*>(P.a + to), l = *reinterpret_cast<const half4*>(P.a + P.na + to);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(C.b, whole(h[e], l[e]), C.c * v[e]);
-    } else if constexpr (KIND == kApply || KIND == kResult) {
-        const half4 h = *reinterpret_cast<const half4*>(P.xt[turn] + to), l = *reinterpret_cast<const half4*>(P.xt[turn] + P.nt + to);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(C.a, whole(h[e], l[e]), v[e]);
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (KIND == kPoly) v[e] = __builtin_fmaf(C.b, whole(old.hi[e], old.lo[e]), C.c * v[e]);
+        else if constexpr (KIND != kGram) v[e] = __builtin_fmaf(C.a, whole(old.hi[e], old.lo[e]), v[e]);
     }
     if constexpr (KIND == kResult) {
 #pragma unroll
@@ -309,8 +322,8 @@ __device__ __forceinline__ void finish_column(const Item& I, const Planes& P, co
     }
     _Float16* o = KIND == kGram ? P.a : KIND == kPoly ? P.b : P.xt[turn ^ 1];
     const int64_t n = KIND == kApply ? P.nt : P.na;
-    *reinterpret_cast<half4*>(o + to) = hi;
-    *reinterpret_cast<half4*>(o + n + to) = lo;
+    put(o + to, hi);
+    put(o + n + to, lo);
 }
 
 // Four columns j .. j + 3 of row i from their words, in row order (X, or the mirror image of a tile off the diagonal).
@@ -324,8 +337,8 @@ __device__ __forceinline__ void finish_row(const Item& I, const Planes& P, int i
     }
     _Float16* o = KIND == kGram ? P.a : KIND == kPoly ? P.b : P.x;
     const int64_t n = KIND == kApply ? P.nx : P.na, at = static_cast<int64_t>(i) * (KIND == kApply ? I.ll : I.ls) + j;
-    *reinterpret_cast<half4*>(o + at) = hi;
-    *reinterpret_cast<half4*>(o + n + at) = lo;
+    put(o + at, hi);
+    put(o + n + at, lo);
 }
 
 // Four columns c .. c + 3 of row r of the result, or of the weight it updates.
@@ -502,11 +515,17 @@ __global__ __launch_bounds__(kWave* kWaves) void ortho_product(const Items* __re
         for (int q = 0; q + 1 < kSteps; ++q) interleave<kProducts, kReads, kShare>();
         interleave<kProducts, 0, kShare>();
     }
+    // what the product adds to, all of it at once: loads between the stores below would wait for one another
+    constexpr int kSide = N * 32, kPasses = kSide * kSide / 4 / kWave, kAcross = kSide / 4;
+    Old old[kPasses];
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x)
+        old[x] = old_values<KIND>(I, P, turn, t.i0 + wi + (x * kWave + lane) % kAcross * 4, t.j0 + wj + (x * kWave + lane) / kAcross);
     meet<0>();                                              // no copy is under way, nobody reads a stage any more
     // The sums go through LDS, a wavefront's block at a time, so that what lies along memory is read and written in runs
     // of its whole side: buf[j][i].  (Straight from the registers, 16 bytes of a line at a time, this cost as much as a
     // third of the products.)  Element e of a block: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32.
-    constexpr int kSide = N * 32, kRow = kSide + 4;
+    constexpr int kRow = kSide + 4;
     static_assert(kWaves * kSide * kRow * sizeof(uint32_t) <= lds_bytes(TILE), "fits the stages");
     uint32_t* buf = reinterpret_cast<uint32_t*>(lds) + wave * kSide * kRow;
 #pragma unroll
@@ -522,14 +541,14 @@ __global__ __launch_bounds__(kWave* kWaves) void ortho_product(const Items* __re
             }
     wave_lds();
     const bool tall = I.rows > I.cols;
-#pragma unroll 4
-    for (int x = lane; x < kSide * kSide / 4; x += kWave) {
-        const int i = x % (kSide / 4) * 4, j = x / (kSide / 4);
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) {
+        const int i = (x * kWave + lane) % kAcross * 4, j = (x * kWave + lane) / kAcross;
         uint32_t w[4];
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(buf[j * kRow + i + e]);
-        finish_column<KIND>(I, P, C, turn, t.i0 + wi + i, t.j0 + wj + j, v, w);
+        finish_column<KIND>(I, P, C, turn, t.i0 + wi + i, t.j0 + wj + j, old[x], v, w);
         if (KIND == kResult && tall) {
             write_result<T>(I, U, t.j0 + wj + j, t.i0 + wi + i, w);
         } else {
@@ -539,9 +558,9 @@ __global__ __launch_bounds__(kWave* kWaves) void ortho_product(const Items* __re
     }
     if (KIND == kResult ? tall : symmetric(KIND) && t.i0 == t.j0) return;      // (a tile on the diagonal is its own mirror image)
     wave_lds();
-#pragma unroll 4
-    for (int x = lane; x < kSide * kSide / 4; x += kWave) {
-        const int j = x % (kSide / 4) * 4, i = x / (kSide / 4);
+#pragma unroll
+    for (int x = 0; x < kPasses; ++x) {
+        const int j = (x * kWave + lane) % kAcross * 4, i = (x * kWave + lane) / kAcross;
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = buf[(j + e) * kRow + i];
@@ -603,7 +622,7 @@ __global__ __launch_bounds__(kWave* kSmallWaves) void ortho_product_small(const 
 #pragma unroll
             for (int x = 1; x < kSmallWaves; ++x) v[e] += part[x][u][f + e];
         }
-        finish_column<KIND>(I, P, C, turn, t.i0 + f, t.j0 + u, v, w);
+        finish_column<KIND>(I, P, C, turn, t.i0 + f, t.j0 + u, old_values<KIND>(I, P, turn, t.i0 + f, t.j0 + u), v, w);
         if (KIND == kResult && tall) write_result<T>(I, U, t.j0 + u, t.i0 + f, w);
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[0][u][f + e] = __uint_as_float(w[e]);
