@@ -20,12 +20,12 @@
 // A list of matrices shares its launches: the tiles of all of them are one grid.
 //
 // Measured (one MI355X, kernel times; rates count the fp16 products done):
-//   2 048 x 2 048 fp32, tiles of 128: gram 49 us (0.56 PFLOP/s, 136 tiles for 256 CUs), poly 53, apply 62 (0.83), planes and
-//   norm 10 + 7.  Of gram's time 15 us are launch, first stage and epilogue; the rest is 1.7 times its matrix instructions
-//   alone and 1.2 times its copies alone, which the L2 gives a CU at 62 GB/s.
-//   8 x 512 x 1 024 bf16: gram 18, poly 11 (tiles of 64), apply 26 (128), planes and norm 17 + 5
-//   333 x 1 001 fp32, tiles of 32: gram 11, poly 5, apply 11.5, planes and norm 7 + 3.5
-//   128 x 602 and 41 x 128 together: gram 6.6, poly 4.3, apply 5.6, planes and norm 5.7 + 4.6: a launch after another, which
+//   2 048 x 2 048 fp32, tiles of 128: gram 48 us (0.57 PFLOP/s, 136 tiles for 256 CUs), poly 49, apply 59 (0.87), planes and
+//   norm 10 + 7.  Without their epilogues 43, 41 and 45; the rest of a tile is 1.7 times its matrix instructions alone and
+//   1.2 times its copies alone, which reach a CU at 62 GB/s.
+//   8 x 512 x 1 024 bf16: gram 17, poly 11 (tiles of 64), apply 24 (128), planes and norm 16 + 5
+//   333 x 1 001 fp32, tiles of 32: gram 11, poly 4.7, apply 11.5, planes and norm 6.5 + 3.5
+//   128 x 602 and 41 x 128 together: gram 6.6, poly 4.3, apply 5.7, planes and norm 5.7 + 4.6: a launch after another, which
 //   neither more wavefronts, loads further ahead, other strides nor fewer loads on the way to a tile make shorter
 //
 // Three shapes of the same product, chosen launch by launch by how many tiles there are (see choose()):
@@ -654,7 +654,7 @@ int64_t tiles_of(const Items& L, bool square, int tile) {
 
 // Tile size of a launch: a larger tile fetches less for its work, but wants half the chip's 256 CUs to have one.
 // Measured, the other choice in brackets: 136 symmetric tiles of 128 (side 2048) 49 us [58]; 80 of them, as 288 tiles of
-// 64 (8 x 512 x 1024) 17.6 us [25.7]; 96 tiles of 64 (333 x 1001) as 352 of 32 11.4 us [11.2].
+// 64 (8 x 512 x 1024), 17.6 us [25.7]; 96 tiles of 64 (333 x 1001) as 352 of 32 11.4 us [11.2].
 constexpr int kFullGrid = 128;
 int choose(const Items& L, bool square) {
     if (tiles_of(L, square, 128) >= kFullGrid) return 128;
