@@ -371,6 +371,28 @@ def test_many_short_graphs_behind_a_long_one(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("first,graphs", [(1100, 2000), (2_190_000, 1)])
+def test_elements_beyond_2_to_the_31(gpu, first, graphs):
+    """The last graph of a batch whose elements pass 2^31, short graphs in one launch and a long one in pieces."""
+    ch, groups, last = 1024, 32, 1100
+    rows = first * graphs + last
+    say("far elements", rows, ch)
+    assert (rows - last) * ch > 1 << 31
+    g = torch.Generator(device=gpu).manual_seed(2)
+    x = torch.randn((rows, ch), generator=g, device=gpu, dtype=BF16).requires_grad_()
+    dy = torch.randn((rows, ch), generator=g, device=gpu, dtype=BF16)
+    w, b = (1 + 0.1 * torch.randn(ch, generator=g, device=gpu)).requires_grad_(), torch.zeros(ch, device=gpu, requires_grad=True)
+    batch = GraphBatch([*range(0, first * graphs + 1, first), rows])
+    y = group_norm(x, groups, w, b, graphs=batch, activation="silu")
+    dx, _, db = torch.autograd.grad(y, (x, w, b), dy)
+    tail = lambda t: t.detach()[-last:].cpu()               # noqa: E731
+    ry, rdx, _, _, ey, edx, _, _ = reference(tail(x), groups, w, b, [0, last], 1e-5, "silu", tail(dy))
+    close(tail(y), ry, ey, BF16, "y")
+    close(tail(dx), rdx, edx, BF16, "dx")
+    assert torch.isfinite(db).all()
+
+
+@pytest.mark.gpu
 def test_a_second_derivative_is_refused(gpu):
     x = torch.randn((40, 8), device=gpu, requires_grad=True)
     dx, = torch.autograd.grad(group_norm(x, 2, activation="silu").sum(), x, create_graph=True)
