@@ -6,6 +6,7 @@
 // backward of 232 965 x 41 labels take 26 us of kernels; issuing them takes 47 us, 96 with nodes in Python (on the same
 // kind of host an empty Python node takes 41); of a norm of 24 001 x 602 in 37 graphs 83 us, 147 in Python; scores
 // without a gradient 9 us, 16 in Python.
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -55,6 +56,14 @@ Tensor rows_of(Tensor t, int64_t width) {
     return t;
 }
 int64_t ld(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : std::max<int64_t>(m.size(1), 1); }
+
+// The operators have no forward-mode derivative: a result without a tangent would be read as a derivative of zero.
+void no_tangents(at::ArrayRef<MaybeTensor> inputs, const char* where) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const MaybeTensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), where,
+                                    " has no forward-mode derivative; torch.autograd differentiates it in reverse mode");
+}
 
 // Gradients have no derivative of their own: where a graph of them is asked for, following it is an error.
 variable_list once(variable_list grads) {
@@ -134,6 +143,7 @@ struct LabelScores : torch::autograd::Function<LabelScores> {
 
 std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> label_scores(const Tensor& z, const MaybeTensor& labels, bool entropy,
                                                                             int64_t top, int64_t ignore_index) {
+    no_tangents({z}, "label_log_probs");
     auto some = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; };
     if (!at::GradMode::is_enabled() || !z.requires_grad()) {
         const Scores s = run_scores(z, labels, entropy, top, ignore_index, false);
@@ -225,6 +235,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 Tensor group_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, const Batch& batch, int64_t groups, double eps,
                   int64_t act) {
+    no_tangents({x, weight, bias}, "group_norm");
     auto grad = [](const MaybeTensor& t) { return t && t->requires_grad(); };
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || grad(weight) || grad(bias)))
         return run_norm(x, weight, bias, batch->rows, groups, eps, act, false).y;
@@ -237,6 +248,9 @@ PYBIND11_MODULE(cbm_autograd, m) {
     const auto unlocked = py::call_guard<py::gil_scoped_release>();
     m.def("label_scores", &label_scores, unlocked);
     m.def("group_norm", &group_norm, unlocked);
+    m.def("no_tangents", [](const std::vector<Tensor>& inputs, const std::string& where) {
+        no_tangents(std::vector<MaybeTensor>(inputs.begin(), inputs.end()), where.c_str());
+    });
     py::class_<NormBatch, Batch>(m, "NormBatch")
         .def(py::init<int64_t, int64_t, int64_t, int64_t, int64_t, variable_list>())
         .def_readonly("arrays", &NormBatch::arrays);

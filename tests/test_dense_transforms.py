@@ -1,0 +1,76 @@
+"""What follows torch's operators cannot follow the dense operators' kernels, which write through raw pointers: where it
+would go on with a wrong result, the calls raise.  The checks run on CPU tensors too, before anything is launched."""
+import sys
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from cbm4gnn_amd import _lib
+from cbm4gnn_amd.labels import label_log_probs
+from cbm4gnn_amd.norm import GroupNorm, group_norm
+from cbm4gnn_amd.optim import muon_step, orthogonalise
+
+
+def say(*a):
+    print("[gpu-case]", *a, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+    return torch.device("cuda", 0)
+
+
+def native(x, labels, weight=None, bias=None):
+    """The two operators' native calls as a list, each of them without the public call's own checks."""
+    lib = _lib.autograd_lib()
+    batch = lib.NormBatch(1, x.size(0), x.size(0), 64, 0, [])
+    return [lambda: lib.group_norm(x, weight, bias, batch, 2, 1e-5, 2), lambda: lib.label_scores(x, labels, True, 2, -100)]
+
+
+FORWARD = "no forward-mode derivative"
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(requires_grad):
+    """Of every differentiable input, whether or not it requires a gradient of its own."""
+    x, w, labels = torch.randn((6, 8)), torch.ones(8), torch.arange(6)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x.clone().requires_grad_(requires_grad), torch.ones_like(x))
+        dual_w = forward_ad.make_dual(w.clone().requires_grad_(requires_grad), torch.ones_like(w))
+        for call in native(dual, labels) + native(x, labels, dual_w)[:1] + native(x, labels, None, dual_w)[:1]:
+            for context in (torch.enable_grad, torch.no_grad):
+                with context(), pytest.raises(RuntimeError, match=FORWARD):
+                    call()
+        with pytest.raises(RuntimeError, match=FORWARD):
+            orthogonalise(dual)
+        for at in range(3):
+            args = [[dual] if i == at else [torch.zeros_like(x)] for i in range(3)]
+            with pytest.raises(RuntimeError, match=FORWARD):
+                muon_step(*args, lr=0.1)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_on_the_gpu_and_ends_with_its_level(gpu):
+    say("forward mode")
+    x, labels = torch.randn((6, 8), device=gpu), torch.arange(6, device=gpu)
+    norm = GroupNorm(2, 8).to(gpu)
+    want = [norm(x), label_log_probs(x, labels).logp, orthogonalise(x)]
+    calls = [norm, lambda t: label_log_probs(t, labels).logp, orthogonalise]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        host = forward_ad.make_dual(x.cpu(), torch.ones_like(x).cpu())
+        for call, plain in zip(calls, want):
+            with pytest.raises(RuntimeError, match=FORWARD):
+                call(dual)
+            assert torch.equal(call(x), plain)              # a tensor without a tangent is as welcome as ever
+            with forward_ad._set_fwd_grad_enabled(False):   # as inside a torch.autograd.Function
+                assert torch.equal(call(dual), plain)
+        for call in (lambda t: group_norm(t, 2), lambda t: label_log_probs(t, labels.cpu())):
+            with pytest.raises(RuntimeError, match=FORWARD):
+                call(host)
+    for call, plain in zip(calls, want):
+        assert torch.equal(call(x), plain)
