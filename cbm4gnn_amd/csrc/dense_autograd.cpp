@@ -8,8 +8,10 @@
 // without a gradient 9 us, 16 in Python.
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -57,8 +59,14 @@ Tensor rows_of(Tensor t, int64_t width) {
 }
 int64_t ld(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : std::max<int64_t>(m.size(1), 1); }
 
-// The operators have no forward-mode derivative: a result without a tangent would be read as a derivative of zero.
-void no_tangents(at::ArrayRef<MaybeTensor> inputs, const char* where) {
+// Refuses what would go on with a wrong result, for the kernels write through raw pointers, unseen by torch:
+//   * forward mode: a result without a tangent would be read as a derivative of zero;
+//   * a tracer (torch.jit.trace, make_fx): of a call it would record the allocation of the result, and nothing that fills it.
+void not_followed(at::ArrayRef<MaybeTensor> inputs, const char* where) {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY), where,
+                                " cannot be traced: a tracer does not see what its kernels write");
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const MaybeTensor& t : inputs)
         TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->defined() || !t->_fw_grad(0).defined(), where,
@@ -143,7 +151,7 @@ struct LabelScores : torch::autograd::Function<LabelScores> {
 
 std::tuple<MaybeTensor, MaybeTensor, MaybeTensor, MaybeTensor> label_scores(const Tensor& z, const MaybeTensor& labels, bool entropy,
                                                                             int64_t top, int64_t ignore_index) {
-    no_tangents({z}, "label_log_probs");
+    not_followed({z}, "label_log_probs");
     auto some = [](const Tensor& t) { return t.defined() ? MaybeTensor(t) : std::nullopt; };
     if (!at::GradMode::is_enabled() || !z.requires_grad()) {
         const Scores s = run_scores(z, labels, entropy, top, ignore_index, false);
@@ -235,7 +243,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 
 Tensor group_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, const Batch& batch, int64_t groups, double eps,
                   int64_t act) {
-    no_tangents({x, weight, bias}, "group_norm");
+    not_followed({x, weight, bias}, "group_norm");
     auto grad = [](const MaybeTensor& t) { return t && t->requires_grad(); };
     if (!at::GradMode::is_enabled() || !(x.requires_grad() || grad(weight) || grad(bias)))
         return run_norm(x, weight, bias, batch->rows, groups, eps, act, false).y;
@@ -248,8 +256,8 @@ PYBIND11_MODULE(cbm_autograd, m) {
     const auto unlocked = py::call_guard<py::gil_scoped_release>();
     m.def("label_scores", &label_scores, unlocked);
     m.def("group_norm", &group_norm, unlocked);
-    m.def("no_tangents", [](const std::vector<Tensor>& inputs, const std::string& where) {
-        no_tangents(std::vector<MaybeTensor>(inputs.begin(), inputs.end()), where.c_str());
+    m.def("not_followed", [](const std::vector<Tensor>& inputs, const std::string& where) {
+        not_followed(std::vector<MaybeTensor>(inputs.begin(), inputs.end()), where.c_str());
     });
     py::class_<NormBatch, Batch>(m, "NormBatch")
         .def(py::init<int64_t, int64_t, int64_t, int64_t, int64_t, variable_list>())

@@ -74,7 +74,7 @@ def orthogonalise(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
             raise ValueError("g: the dimensions before the last two must collapse into one") from None
     if mats:
         _check_matrix(mats[0], "g")
-    _lib.autograd_lib().no_tangents([g], "orthogonalise")   # torch.no_grad leaves the forward mode on
+    _lib.autograd_lib().not_followed([g], "orthogonalise")    # torch.no_grad leaves the forward mode on
     _require_gpu()
     if not g.is_cuda:
         return orthogonalise(g.to("cuda"), steps, coefficients, eps).to(g.device)
@@ -125,7 +125,7 @@ def muon_step(weights, grads, buffers, *, lr, momentum=0.95, weight_decay=0.0, n
             seen.add(t.data_ptr())
         if g.numel() and g.data_ptr() in (w.data_ptr(), b.data_ptr()):
             raise ValueError("a gradient must not be its weight or momentum buffer")
-    _lib.autograd_lib().no_tangents(weights + grads + buffers, "muon_step")
+    _lib.autograd_lib().not_followed(weights + grads + buffers, "muon_step")
     _require_gpu()
     dev = weights[0].device
     if dev.type != "cuda":

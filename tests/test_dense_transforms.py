@@ -5,6 +5,7 @@ import sys
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from cbm4gnn_amd import _lib
 from cbm4gnn_amd.labels import label_log_probs
@@ -32,6 +33,12 @@ def native(x, labels, weight=None, bias=None):
 
 
 FORWARD = "no forward-mode derivative"
+TRACED = "cannot be traced"
+
+
+def tracers():
+    """Ways to trace f(x)."""
+    return [lambda f, x: torch.jit.trace(f, x, check_trace=False), lambda f, x: make_fx(f)(x), lambda f, x: make_fx(f, tracing_mode="fake")(x)]
 
 
 @pytest.mark.parametrize("requires_grad", [False, True])
@@ -74,3 +81,41 @@ def test_forward_mode_is_refused_on_the_gpu_and_ends_with_its_level(gpu):
                 call(host)
     for call, plain in zip(calls, want):
         assert torch.equal(call(x), plain)
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_tracing_is_refused(requires_grad):
+    """A trace would hold the allocation of the result and nothing that fills it."""
+    x, labels = torch.randn((6, 8)).requires_grad_(requires_grad), torch.arange(6)
+
+    def muon(t):
+        muon_step([t], [t + 1], [t + 2], lr=0.1)
+        return t
+    for trace in tracers():
+        for k in range(2):
+            for context in (torch.enable_grad, torch.no_grad):
+                with context(), pytest.raises(RuntimeError, match=TRACED):
+                    trace(lambda t: native(t, labels)[k](), x)
+        with pytest.raises(RuntimeError, match=TRACED):
+            trace(lambda t: orthogonalise(t), x)
+        with pytest.raises(RuntimeError, match=TRACED + "|data pointer"):      # (a fake tensor has no memory to check for overlaps)
+            trace(muon, x)
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_is_refused_on_the_gpu_and_ends_with_its_trace(gpu):
+    say("tracing")
+    x, labels = torch.randn((6, 8), device=gpu), torch.arange(6, device=gpu)
+    calls = [GroupNorm(2, 8).to(gpu), lambda t: label_log_probs(t, labels, entropy=True)[:2], lambda t: orthogonalise(t)]
+    for trace in tracers()[:2]:
+        for call in calls:
+            want = call(x)
+            with pytest.raises(RuntimeError, match=TRACED):
+                trace(call, x)
+            for p, q in zip(want, call(x)):
+                assert torch.equal(p, q)
+        for call in (lambda t: group_norm(t, 2), lambda t: label_log_probs(t, labels.cpu()).logp):
+            with pytest.raises(RuntimeError, match=TRACED):
+                trace(call, x.cpu())
