@@ -136,6 +136,17 @@ inline int check_launch() { return hipGetLastError() == hipSuccess ? CBM_OK : CB
 
 inline int element_bytes(int dtype) { return dtype == CBM_DTYPE_F32 ? 4 : 2; }
 
+// Whether two matrices [rows, width] of e-byte elements share memory.  Rows of one stride may interleave; those of different
+// strides are taken to meet where their ranges do.
+inline bool overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t width, int e) {
+    if (!a || !b || rows < 1) return false;
+    const int64_t d = reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a), w = width * e, s = lda * e;
+    if (d >= (rows - 1) * s + w || -d >= (rows - 1) * ldb * e + w) return false;
+    if (lda != ldb || rows == 1) return true;
+    const int64_t q = d >= 0 ? d / s : -((-d + s - 1) / s), m = d - q * s;       // row i of b begins m bytes into row i + q of a
+    return (m < w && q < rows && -q < rows) || (s - m < w && q + 1 < rows && -(q + 1) < rows);
+}
+
 }  // namespace cbm_dense
 
 #endif

@@ -663,6 +663,7 @@ int cbm_label_scores_backward(const void* logits, const int64_t* labels, const f
                               int32_t top, int64_t ld, int64_t ldg, int64_t ignore_index, int32_t dtype, void* stream) {
     if (int rc = check_labels(rows, classes, top, ld, dtype)) return rc;
     if (ldg < classes) return CBM_ERR_SHAPE;
+    if (overlap(logits, ld, grad, ldg, rows, classes, element_bytes(dtype))) return CBM_ERR_SHAPE;     // read again while it is written
     if (rows == 0) return CBM_OK;
     if (!logits || !stats || !grad || (g_logp && !labels) || (g_entropy && !entropy) || (g_top && (!top_index || top < 1)))
         return CBM_ERR_NULL;

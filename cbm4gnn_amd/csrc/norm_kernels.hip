@@ -964,6 +964,9 @@ int cbm_group_norm_forward(const cbm_norm_batch* B, const void* X, void* Y, cons
     if (B->rows == 0) return CBM_OK;
     if (!X || !Y) return CBM_ERR_NULL;
     if (ldx < C || ldy < C || !(eps >= 0.f)) return CBM_ERR_SHAPE;
+    // Both directions read their inputs again after others have begun to write, and two threads share the channels where a
+    // row's last vector overlaps the one before.
+    if (overlap(X, ldx, Y, ldy, B->rows, C, element_bytes(dtype))) return CBM_ERR_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     Plan P = plan_of(B, C, groups, dtype, false);
     Shape& S = P.S;
@@ -1009,6 +1012,8 @@ int cbm_group_norm_backward(const cbm_norm_batch* B, const void* X, const void* 
     if (int rc = check_batch(B, C, groups, dtype, act)) return rc;
     if (B->rows > 0 && (!X || !DY || !mean || !rstd)) return CBM_ERR_NULL;
     if (ldx < C || ldg < C || (DX && ldd < C)) return CBM_ERR_SHAPE;
+    if (overlap(X, ldx, DX, ldd, B->rows, C, element_bytes(dtype)) || overlap(DY, ldg, DX, ldd, B->rows, C, element_bytes(dtype)))
+        return CBM_ERR_SHAPE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool params = dweight || dbias;
     if (!params && (!DX || B->rows == 0)) return CBM_OK;

@@ -614,7 +614,8 @@ int csr_spmm_f32(const int32_t* rowptr_dev, const int32_t* col_dev, int64_t nnz,
  * labels, update of the weights.  The reference leaves all three to torch (its benchmark model has a
  * ReLU between the layers and nothing else, benchmark/parallel/benchmark_gcn_cpu.py:62-89).  Same
  * conventions as above: device pointers, row strides in elements, caller-owned workspace, no
- * allocation, no synchronisation, a status for an answer.  Sums and statistics are fp32.
+ * allocation, no synchronisation, a status for an answer.  Sums and statistics are fp32.  No result may
+ * share memory with an input: Y, DX and grad are refused (CBM_ERR_SHAPE) where they overlap X, DY or logits.
  * ------------------------------------------------------------------------------------------------- */
 enum { CBM_DTYPE_F32 = 0, CBM_DTYPE_BF16 = 1, CBM_DTYPE_F16 = 2 };   /* elements of X, Y, logits, matrices */
 enum { CBM_ACT_NONE = 0, CBM_ACT_RELU = 1, CBM_ACT_SILU = 2 };
@@ -642,7 +643,7 @@ int cbm_group_norm_forward(const cbm_norm_batch* batch, const void* X_dev, void*
                            const float* bias_dev, float* mean_dev, float* rstd_dev, float* workspace_dev, int32_t C,
                            int32_t groups, int64_t ldx, int64_t ldy, float eps, int32_t act, int32_t dtype, void* stream);
 /* Gradients for DY [rows, C]: DX (nullable), dweight and dbias (nullable; zero where the batch has no rows).
- * DX may be DY.  workspace: cbm_group_norm_workspace_floats(.., backward = 1) floats. */
+ * workspace: cbm_group_norm_workspace_floats(.., backward = 1) floats. */
 int cbm_group_norm_backward(const cbm_norm_batch* batch, const void* X_dev, const void* DY_dev, void* DX_dev,
                             const float* weight_dev, const float* bias_dev, const float* mean_dev, const float* rstd_dev,
                             float* dweight_dev, float* dbias_dev, float* workspace_dev, int32_t C, int32_t groups,
