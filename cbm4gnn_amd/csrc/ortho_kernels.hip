@@ -212,8 +212,8 @@ __global__ __launch_bounds__(256) void ortho_split(const Items* __restrict__ lis
     for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = sum;
     __syncthreads();
-    // in 64 bits: neither a norm beyond fp32 nor the reciprocal of a tiny one costs anything
-    const double inv = 1.0 / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + static_cast<double>(eps));
+    // in 64 bits: neither a norm beyond fp32 nor the reciprocal of a tiny one costs anything; zeros stay zeros without an eps too
+    const double size = sqrt((red[0] + red[1]) + (red[2] + red[3])) + static_cast<double>(eps), inv = size == 0.0 ? 0.0 : 1.0 / size;
 #pragma unroll
     for (int y = 0; y < 16; ++y) tile[tall ? tx : ty + 4 * y][tall ? ty + 4 * y : tx] = static_cast<float>(v[y] * inv);     // [short][long]
     __syncthreads();
