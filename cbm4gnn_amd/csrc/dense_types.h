@@ -136,15 +136,21 @@ inline int check_launch() { return hipGetLastError() == hipSuccess ? CBM_OK : CB
 
 inline int element_bytes(int dtype) { return dtype == CBM_DTYPE_F32 ? 4 : 2; }
 
-// Whether two matrices [rows, width] of e-byte elements share memory.  Rows of one stride may interleave; those of different
-// strides are taken to meet where their ranges do.
+// A matrix of e-byte elements in memory, and whether two of them share any.  Rows of one stride may interleave; those of
+// different strides are taken to meet where their ranges do.
+struct Extent { const void* at; int64_t ld, rows, width; };
+inline bool overlap(Extent a, Extent b, int e) {
+    if (!a.at || !b.at || a.rows < 1 || b.rows < 1) return false;
+    if (a.rows == 1) a.ld = b.ld;
+    if (b.rows == 1) b.ld = a.ld;
+    const int64_t d = reinterpret_cast<intptr_t>(b.at) - reinterpret_cast<intptr_t>(a.at), s = a.ld * e, wa = a.width * e, wb = b.width * e;
+    if (d >= (a.rows - 1) * s + wa || -d >= (b.rows - 1) * b.ld * e + wb) return false;
+    if (a.ld != b.ld || (a.rows == 1 && b.rows == 1)) return true;
+    const int64_t q = d >= 0 ? d / s : -((-d + s - 1) / s), m = d - q * s;       // row j of b begins m bytes into row j + q of a
+    return (m < wa && q < a.rows && -q < b.rows) || (s - m < wb && q + 1 < a.rows && -(q + 1) < b.rows);
+}
 inline bool overlap(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t rows, int64_t width, int e) {
-    if (!a || !b || rows < 1) return false;
-    const int64_t d = reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a), w = width * e, s = lda * e;
-    if (d >= (rows - 1) * s + w || -d >= (rows - 1) * ldb * e + w) return false;
-    if (lda != ldb || rows == 1) return true;
-    const int64_t q = d >= 0 ? d / s : -((-d + s - 1) / s), m = d - q * s;       // row i of b begins m bytes into row i + q of a
-    return (m < w && q < rows && -q < rows) || (s - m < w && q + 1 < rows && -(q + 1) < rows);
+    return overlap(Extent{a, lda, rows, width}, Extent{b, ldb, rows, width}, e);
 }
 
 }  // namespace cbm_dense

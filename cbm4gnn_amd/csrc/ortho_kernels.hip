@@ -38,6 +38,9 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <functional>
+#include <memory>
+#include <new>
 
 #include "dense_types.h"
 
@@ -749,7 +752,36 @@ int run_turn(const cbm_ortho_item* items, int n, const Update& U, int steps, con
 
 constexpr int kMaxSide = 1 << 20;
 
-int check_items(const cbm_ortho_item* items, int n, bool update) {
+// Whether what a call writes meets anything else of its list: the items share launches, so their order is open.  By address,
+// each matrix is held against those that begin before it ends.
+int check_apart(const cbm_ortho_item* items, int n, bool update, int e) {
+    struct Matrix { Extent x; intptr_t end; bool written; };
+    const std::unique_ptr<Matrix[]> all(new (std::nothrow) Matrix[3 * static_cast<size_t>(n)]);
+    if (!all) return CBM_ERR_ALLOC;
+    int m = 0;
+    auto add = [&](const cbm_ortho_item& s, const void* at, int64_t ld, bool written) {
+        const Extent x{at, ld, s.rows, s.cols};
+        all[m++] = {x, reinterpret_cast<intptr_t>(at) + ((s.rows - 1) * ld + s.cols) * e, written};
+    };
+    for (int i = 0; i < n; ++i) {
+        const cbm_ortho_item& s = items[i];
+        if (s.rows == 0 || s.cols == 0) continue;
+        add(s, s.src, s.ld_src, false);
+        if (update) {
+            add(s, s.weight, s.ld_weight, true);
+            add(s, s.momentum, s.ld_momentum, true);
+        } else {
+            add(s, s.dst, s.ld_dst, true);
+        }
+    }
+    std::sort(all.get(), all.get() + m, [](const Matrix& a, const Matrix& b) { return std::less<const void*>()(a.x.at, b.x.at); });
+    for (int i = 0; i < m; ++i)
+        for (int j = i + 1; j < m && reinterpret_cast<intptr_t>(all[j].x.at) < all[i].end; ++j)
+            if ((all[i].written || all[j].written) && overlap(all[i].x, all[j].x, e)) return CBM_ERR_SHAPE;
+    return CBM_OK;
+}
+
+int check_items(const cbm_ortho_item* items, int n, bool update, int e) {
     if (n < 0) return CBM_ERR_SHAPE;
     if (n > 0 && !items) return CBM_ERR_NULL;
     for (int i = 0; i < n; ++i) {
@@ -759,7 +791,7 @@ int check_items(const cbm_ortho_item* items, int n, bool update) {
         if (!s.src || (update ? !s.weight || !s.momentum : !s.dst)) return CBM_ERR_NULL;
         if (s.ld_src < s.cols || (update ? s.ld_weight < s.cols || s.ld_momentum < s.cols : s.ld_dst < s.cols)) return CBM_ERR_SHAPE;
     }
-    return CBM_OK;
+    return check_apart(items, n, update, e);
 }
 
 template <typename T>
@@ -786,8 +818,9 @@ int64_t cbm_ortho_workspace_bytes(const cbm_ortho_item* items, int32_t n) {
 
 int cbm_orthogonalise(const cbm_ortho_item* items, int32_t n, int32_t steps, float a, float b, float c, float eps, int32_t dtype,
                       void* workspace, void* stream) {
-    if (int rc = check_items(items, n, false)) return rc;
-    if (steps < 1 || !(eps >= 0.f) || dtype < CBM_DTYPE_F32 || dtype > CBM_DTYPE_F16) return CBM_ERR_SHAPE;
+    if (dtype < CBM_DTYPE_F32 || dtype > CBM_DTYPE_F16) return CBM_ERR_SHAPE;
+    if (int rc = check_items(items, n, false, element_bytes(dtype))) return rc;
+    if (steps < 1 || !(eps >= 0.f)) return CBM_ERR_SHAPE;
     if (n > 0 && !workspace && cbm_ortho_workspace_bytes(items, n) > 0) return CBM_ERR_NULL;
     const Update U{0.f, 0.f, 0.f, 0, 0};
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -798,7 +831,7 @@ int cbm_orthogonalise(const cbm_ortho_item* items, int32_t n, int32_t steps, flo
 
 int cbm_muon_step(const cbm_ortho_item* items, int32_t n, float lr, float mu, float decay, int32_t nesterov, int32_t steps, float a,
                   float b, float c, float eps, void* workspace, void* stream) {
-    if (int rc = check_items(items, n, true)) return rc;
+    if (int rc = check_items(items, n, true, sizeof(float))) return rc;
     if (steps < 1 || !(eps >= 0.f)) return CBM_ERR_SHAPE;
     if (n > 0 && !workspace && cbm_ortho_workspace_bytes(items, n) > 0) return CBM_ERR_NULL;
     const Update U{lr, mu, decay, nesterov, 1};

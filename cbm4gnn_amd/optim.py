@@ -99,8 +99,8 @@ def orthogonalise(g, steps=5, coefficients=NS_COEFFICIENTS, eps=1e-7):
 def muon_step(weights, grads, buffers, *, lr, momentum=0.95, weight_decay=0.0, nesterov=True, steps=5,
               coefficients=NS_COEFFICIENTS, eps=1e-7):
     """One step over lists of float32 matrices on one GPU: ``buffers`` (momentum, zeros in the beginning) and
-    ``weights`` are updated in place, in launches that all of them share.  No two of the tensors that are written
-    may overlap."""
+    ``weights`` are updated in place, in launches that all of them share: neither may overlap any other tensor of the
+    step (a gradient may be given twice)."""
     steps, abc, eps = _check_steps(steps, coefficients, eps)
     weights, grads, buffers = list(weights), list(grads), list(buffers)
     if not len(weights) == len(grads) == len(buffers):
@@ -123,8 +123,8 @@ def muon_step(weights, grads, buffers, *, lr, momentum=0.95, weight_decay=0.0, n
             if t.numel() and t.data_ptr() in seen:
                 raise ValueError("the same weight or momentum buffer is given twice")
             seen.add(t.data_ptr())
-        if g.numel() and g.data_ptr() in (w.data_ptr(), b.data_ptr()):
-            raise ValueError("a gradient must not be its weight or momentum buffer")
+    if any(g.numel() and g.data_ptr() in seen for g in grads):
+        raise ValueError("a gradient must not be a weight or momentum buffer of the step")
     _lib.autograd_lib().not_followed(weights + grads + buffers, "muon_step")
     _require_gpu()
     dev = weights[0].device

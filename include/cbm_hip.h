@@ -672,12 +672,13 @@ int cbm_label_scores_backward(const void* logits_dev, const int64_t* labels_dev,
 /* Newton-Schulz orthogonalisation of matrices G [rows, cols], and the optimiser step around it:
  *   X = G / (|G|_F + eps);  `steps` times: X = a X + (b A + c A A) X with A = X X^T  (taken on the shorter side)
  * A list of matrices of any shapes shares its launches; up to CBM_ORTHO_MAX_ITEMS go together, longer lists in
- * turns.  The products run on the matrix cores with every operand split into two halves of 11 bits (see
+ * turns.  What a call writes (dst, or weight and momentum) shares memory with no other matrix of its list, or the
+ * call is refused (CBM_ERR_SHAPE).  The products run on the matrix cores with every operand split into two halves of 11 bits (see
  * ortho_kernels.hip), sums in fp32; an item of zeros gives zeros. */
 enum { CBM_ORTHO_MAX_ITEMS = 24 };
 typedef struct cbm_ortho_item {
     const void* src;         /* G [rows, cols], dtype; in cbm_muon_step the gradient, fp32            */
-    void* dst;               /* cbm_orthogonalise: result [rows, cols], dtype, not src                 */
+    void* dst;               /* cbm_orthogonalise: result [rows, cols], dtype                          */
     float* weight;           /* cbm_muon_step: fp32 weight, updated                                    */
     float* momentum;         /* cbm_muon_step: fp32 momentum buffer, updated                           */
     int32_t rows, cols;
