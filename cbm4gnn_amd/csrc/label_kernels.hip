@@ -211,12 +211,14 @@ struct Grads {
 };
 
 // What a row's gradient needs: dz_j = -p_j (all + gh (log p_j + h)) + gl [j = label] (+ the likeliest classes').
-// A row of -inf alone has no gradient.
+// A row of -inf alone has no gradient (any = false), and neither has one whose label is ignored and to which nothing else
+// flows: a row that is left out may hold NaN or +inf, which times zero would be NaN.
 struct RowGrad { float m, log_s, h, gl, gh, all; int label; bool any; };
 __device__ __forceinline__ RowGrad row_grad(const Grads& G, int64_t r) {
     const float2 st = *reinterpret_cast<const float2*>(G.stats + 2 * r);
     RowGrad R{st.x, st.y, 0.f, 0.f, 0.f, 0.f, -1, st.y != kInf};
     if (!R.any) return R;
+    bool left_out = false;
     if (G.g_entropy) { R.gh = G.g_entropy[r]; R.h = G.entropy[r]; }
     if (G.g_logp) {
         const int64_t y = G.labels[r];
@@ -225,11 +227,18 @@ __device__ __forceinline__ RowGrad row_grad(const Grads& G, int64_t r) {
             const bool in = y >= 0 && y < G.classes;
             R.gl = in ? g : __builtin_nanf("");
             R.label = in ? static_cast<int>(y) : -1;
+        } else {
+            left_out = R.gh == 0.f;
         }
     }
     R.all = R.gl;
     if (G.g_top)
-        for (int i = 0; i < G.top; ++i) R.all += G.g_top[r * G.top + i];
+        for (int i = 0; i < G.top; ++i) {
+            const float g = G.g_top[r * G.top + i];
+            R.all += g;
+            left_out = left_out && g == 0.f;
+        }
+    if (left_out) R.any = false;
     return R;
 }
 template <bool H>
@@ -269,10 +278,10 @@ __global__ __launch_bounds__(kThreads) void label_grads_narrow(const T* __restri
         const int at = j < NV - 1 ? (lane + L * j) * V : last.at;
         if (G.g_entropy) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[j][i] = grad_of<true>(R, v[j][i], at + i);
+            for (int i = 0; i < V; ++i) v[j][i] = R.any ? grad_of<true>(R, v[j][i], at + i) : 0.f;
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[j][i] = grad_of<false>(R, v[j][i], at + i);
+            for (int i = 0; i < V; ++i) v[j][i] = R.any ? grad_of<false>(R, v[j][i], at + i) : 0.f;
         }
     }
     if (likeliest)
@@ -478,6 +487,12 @@ __global__ __launch_bounds__(kThreads) void label_grads_wide(const T* __restrict
     const RowGrad R = row_grad(G, r);
     const bool h = G.g_entropy != nullptr;
     const int full = (hi - lo) / V;
+    if (!R.any) {                                           // the same for the whole workgroup
+        const float zeros[V] = {};
+        for (int i = threadIdx.x; i < full; i += kThreads) store_from_f32<T, V>(out + lo + i * V, zeros);
+        if (lo + full * V + static_cast<int>(threadIdx.x) < hi) out[lo + full * V + threadIdx.x] = static_cast<T>(0.f);
+        return;
+    }
 #pragma unroll 2
     for (int i = threadIdx.x; i < full; i += kThreads) {
         const int c = lo + i * V;
@@ -489,7 +504,7 @@ __global__ __launch_bounds__(kThreads) void label_grads_wide(const T* __restrict
     }
     const int c = lo + full * V + threadIdx.x;
     if (c < hi) out[c] = static_cast<T>(grad_of<true>(R, static_cast<float>(row[c]), c));
-    if (!G.g_top || !R.any) return;                         // the same for the whole workgroup
+    if (!G.g_top) return;
     __syncthreads();                                        // the stores above are over: these few go on top of them
     if (static_cast<int>(threadIdx.x) < G.top) {
         const int64_t at = G.top_index[r * G.top + threadIdx.x];

@@ -40,7 +40,8 @@ def label_log_probs(logits, labels=None, *, entropy=False, top=0, ignore_index=-
     NaN counts as the largest.
 
     A row of -inf alone has log probabilities -inf, entropy 0 and no gradient; a NaN or +inf makes the scores of
-    its row NaN.  Logits need unit stride along the classes, rows may be any stride apart."""
+    its row NaN, and their gradients.  A row whose label is ignored may hold either: it scores 0, and its gradient is 0
+    where that of its entropy and of its likeliest classes is.  Logits need unit stride along the classes, rows may be any stride apart."""
     check_dtype(logits, "logits")
     z = rows_view(logits, "logits")
     rows, classes = z.shape

@@ -663,7 +663,8 @@ int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t
 int cbm_label_scores(const void* logits_dev, const int64_t* labels_dev, float* logp_dev, float* entropy_dev, float* top_logp_dev,
                      int64_t* top_index_dev, float* stats_dev, float* workspace_dev, int32_t rows, int32_t classes, int32_t top,
                      int64_t ld, int64_t ignore_index, int32_t dtype, void* stream);
-/* grad [rows, classes] of dtype, from the gradients of logp, entropy (which then is given too) and top_logp, each nullable. */
+/* grad [rows, classes] of dtype, from the gradients of logp, entropy (which then is given too) and top_logp, each nullable.
+ * Zero in the rows whose label is ignored and whose other gradients are zero, whatever their logits hold. */
 int cbm_label_scores_backward(const void* logits_dev, const int64_t* labels_dev, const float* stats_dev, const float* entropy_dev,
                               const int64_t* top_index_dev, const float* g_logp_dev, const float* g_entropy_dev,
                               const float* g_top_dev, void* grad_dev, int32_t rows, int32_t classes, int32_t top, int64_t ld,
