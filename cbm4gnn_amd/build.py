@@ -2,7 +2,7 @@
 
     libcbm_hip.so    hipcc, gfx950 only: the HIP kernels and their C-ABI launchers
     libcbm_host.so   g++ / OpenMP: the host-side format builder
-    cbm_autograd.so  g++ against torch: the dense operators' autograd nodes, over libcbm_hip.so
+    cbm_autograd.so  g++ against torch, where it is installed: the dense operators' autograd nodes, over libcbm_hip.so
 
 Run ``python -m cbm4gnn_amd.build`` (no GPU needed: hipcc cross-compiles).  The reference builds
 its extension with cmake + setuptools against MKL and arbok (``cbm/setup.py:15-47``); none of
@@ -10,6 +10,7 @@ that applies here.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
@@ -87,13 +88,22 @@ def build_autograd(verbose: bool = False) -> str:
 
 
 def build_all(verbose: bool = False):
-    """Side by side, but for what is linked to another."""
+    """The two C-ABI libraries, which need no torch, and, where there is one to compile against, the autograd module
+    (``AUTOGRAD_LIB``).  Side by side, but for what is linked to another.  Returns the paths of the first two."""
     with ThreadPoolExecutor(1) as pool:
-        host = pool.submit(build_host, verbose)
-        return build_hip(verbose), build_autograd(verbose), host.result()
+        pending = pool.submit(build_host, verbose)
+        hip = build_hip(verbose)
+        host = pending.result()
+        if importlib.util.find_spec("torch") is not None:
+            build_autograd(verbose)
+    return hip, host
 
 
 if __name__ == "__main__":
     for p in build_all(verbose=True):
         print("built", p)
+    if importlib.util.find_spec("torch") is not None:
+        print("built", AUTOGRAD_LIB)
+    else:
+        print("no torch: without", AUTOGRAD_LIB)
     sys.exit(0)
