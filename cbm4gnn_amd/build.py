@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -66,6 +67,16 @@ def build_host(verbose: bool = False) -> str:
     return HOST_LIB
 
 
+def _hip_headers() -> str:
+    """The include directory of the ROCm that the compiler belongs to, wherever ``HIPCC`` says that is."""
+    found = shutil.which(HIPCC)
+    roots = [os.path.dirname(os.path.dirname(p)) for p in ((found, os.path.realpath(found)) if found else ())]
+    for root in (*roots, os.environ.get("ROCM_PATH", ""), "/opt/rocm"):
+        if root and os.path.exists(os.path.join(root, "include", "hip", "hip_runtime_api.h")):
+            return os.path.join(root, "include")
+    raise RuntimeError(f"no HIP headers beside {HIPCC}, under ROCM_PATH or in /opt/rocm")
+
+
 def build_autograd(verbose: bool = False) -> str:
     """After ``build_hip``, whose library it is linked to."""
     import sysconfig
@@ -74,11 +85,10 @@ def build_autograd(verbose: bool = False) -> str:
 
     root = os.path.dirname(torch.__file__)
     include, libs = os.path.join(root, "include"), os.path.join(root, "lib")
-    rocm = os.path.dirname(os.path.dirname(HIPCC))
     out = _run(["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                 f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                 *(f"-isystem{d}" for d in (include, os.path.join(include, "torch", "csrc", "api", "include"),
-                                           sysconfig.get_paths()["include"], os.path.join(rocm, "include"))),
+                                           sysconfig.get_paths()["include"], _hip_headers())),
                 "-o", AUTOGRAD_LIB, os.path.join(SRC_DIR, "dense_autograd.cpp"),
                 f"-L{LIB_DIR}", "-l:libcbm_hip.so", "-Wl,-rpath,$ORIGIN",
                 f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"])

@@ -44,3 +44,19 @@ def test_a_failure_is_not_swallowed(commands, monkeypatch):
             m.setattr(build, name, fail)
             with pytest.raises(RuntimeError, match="no compiler"):
                 build.build_all()
+
+
+def test_the_compiler_from_the_path(commands, monkeypatch, tmp_path):
+    """``HIPCC=hipcc``, a link to it, or a wrapper somewhere else: the headers are found all the same."""
+    (tmp_path / "hipcc").symlink_to(build.HIPCC)
+    wrapper = tmp_path / "wrapped" / "hipcc"
+    wrapper.parent.mkdir()
+    wrapper.write_text("#!/bin/sh\n")
+    wrapper.chmod(0o755)
+    monkeypatch.setenv("PATH", f"{tmp_path}:{os.environ['PATH']}")
+    for name in ("hipcc", str(tmp_path / "hipcc"), str(wrapper)):
+        monkeypatch.setattr(build, "HIPCC", name)
+        commands.clear()
+        build.build_autograd()
+        dirs = [part[len("-isystem"):] for part in commands[0] if part.startswith("-isystem")]
+        assert any(os.path.exists(os.path.join(d, "hip", "hip_runtime_api.h")) for d in dirs), name
