@@ -194,6 +194,7 @@ HIP_SYMBOLS = {
     "cbm_label_scores": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I32, _P]),
     "cbm_label_scores_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I64, _I64, _I64, _I32, _P]),
     "cbm_ortho_workspace_bytes": (C.c_int64, [_P, _I32]),
+    "cbm_ortho_tiles": (C.c_int, [_P, _I32, _P, _P]),
     "cbm_orthogonalise": (C.c_int, [_P, _I32, _I32, _F32, _F32, _F32, _F32, _I32, _P, _P]),
     "cbm_muon_step": (C.c_int, [_P, _I32, _F32, _F32, _F32, _I32, _I32, _F32, _F32, _F32, _F32, _P, _P]),
     "cbm_row_intersections_groups": (C.c_int, []),

@@ -816,6 +816,17 @@ int64_t cbm_ortho_workspace_bytes(const cbm_ortho_item* items, int32_t n) {
     return most ? kListBytes + kNormBytes + most * static_cast<int64_t>(sizeof(_Float16)) : 0;
 }
 
+int cbm_ortho_tiles(const cbm_ortho_item* items, int32_t n, int32_t* square, int32_t* wide) {
+    if (!square || !wide || (n > 0 && !items)) return CBM_ERR_NULL;
+    if (n < 0) return CBM_ERR_SHAPE;
+    Items L;
+    Choice choice;
+    lay_out(items, std::min<int>(n, kMaxItems), L, choice);
+    *square = L.n ? choice.square : 0;
+    *wide = L.n ? choice.wide : 0;
+    return CBM_OK;
+}
+
 int cbm_orthogonalise(const cbm_ortho_item* items, int32_t n, int32_t steps, float a, float b, float c, float eps, int32_t dtype,
                       void* workspace, void* stream) {
     if (dtype < CBM_DTYPE_F32 || dtype > CBM_DTYPE_F16) return CBM_ERR_SHAPE;

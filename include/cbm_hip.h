@@ -687,6 +687,9 @@ typedef struct cbm_ortho_item {
 } cbm_ortho_item;
 
 int64_t cbm_ortho_workspace_bytes(const cbm_ortho_item* items, int32_t n_items);
+/* Sides (32, 64 or 128; 0: nothing to do) of the tiles that the symmetric products of the first CBM_ORTHO_MAX_ITEMS items are
+ * cut into, and the others.  From the shapes alone; host only. */
+int cbm_ortho_tiles(const cbm_ortho_item* items, int32_t n_items, int32_t* square, int32_t* wide);
 int cbm_orthogonalise(const cbm_ortho_item* items, int32_t n_items, int32_t steps, float a, float b, float c, float eps,
                       int32_t dtype, void* workspace_dev, void* stream);
 /* momentum = mu momentum + G;  U = G + mu momentum (nesterov) or momentum;  O = orthogonalised U;
