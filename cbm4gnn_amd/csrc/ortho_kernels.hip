@@ -655,13 +655,29 @@ int64_t tiles_of(const Items& L, bool square, int tile) {
     return n;
 }
 
-// Tile size of a launch: a larger tile fetches less for its work, but wants half the chip's 256 CUs to have one.
-// Measured, the other choice in brackets: 136 symmetric tiles of 128 (side 2048) 49 us [58]; 80 of them, as 288 tiles of
-// 64 (8 x 512 x 1024), 17.6 us [25.7]; 96 tiles of 64 (333 x 1001) as 352 of 32 11.4 us [11.2].
+// Operations of the list with sides padded to whole tiles, up to a factor.
+double padded_work(const Items& L, int tile) {
+    double n = 0.0;
+    for (int i = 0; i < L.n; ++i) {
+        const double s = padded(L.it[i].sp, tile), l = padded(L.it[i].lp, tile);
+        n += s * s * l;
+    }
+    return n;
+}
+
+// Tile size of a launch: a larger tile fetches less for its work, but wants half the chip's 256 CUs to have one, and pads
+// every side to itself, work and workspace with it.  How much padding it may bring is measured, whole optimiser steps in us,
+// the smaller tile in brackets.  128 for 64, up to a quarter more work: 4 x 200 x 4096 (none) 308 [319], 12 x 96 x 8192 (none)
+// 615 [640], 8 x 80 x 2048 (none) 195 [172];  3 x 300 x 4096 (1.44) 402 [332], 24 x 130 x 1030 (1.78) 301 [243], 8 x 64 x 2048
+// (4) 197 [155].  64 for 32, up to twice the work: 8 x 40 x 2048 (none) 154 [176], 8 x 130 x 2048 (1.44) 208 [259], 8 x 80 x
+// 2048 (1.78) 172 [201];  8 x 16 x 2048 (4) 151 [151] in 12 MiB of workspace [6], 1 x 2^20 (4) 78.0 ms [72.0].
+// By the number of tiles, launches in us: 136 symmetric tiles of 128 (side 2048) 49 [58 as 64]; 80 of them, as 288 tiles of 64
+// (8 x 512 x 1024), 17.6 [25.7 as 128].  At 96 tiles of 64 (333 x 1001) 64 and 32 are even (11.2, 11.4).
 constexpr int kFullGrid = 128;
 int choose(const Items& L, bool square) {
-    if (tiles_of(L, square, 128) >= kFullGrid) return 128;
-    return tiles_of(L, square, 64) >= kFullGrid ? 64 : 32;
+    const double least = padded_work(L, 32), middle = padded_work(L, 64);
+    if (tiles_of(L, square, 128) >= kFullGrid && padded_work(L, 128) <= 1.25 * middle && middle <= 2.0 * least) return 128;
+    return tiles_of(L, square, 64) >= kFullGrid && middle <= 2.0 * least ? 64 : 32;
 }
 
 // Sides of the items of one turn; halves of workspace they need.  All sides are padded to the larger tile in use.

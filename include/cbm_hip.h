@@ -686,6 +686,8 @@ typedef struct cbm_ortho_item {
     int64_t ld_src, ld_dst, ld_weight, ld_momentum;
 } cbm_ortho_item;
 
+/* 12 rows cols + 8 min(rows, cols)^2 bytes an item, sides rounded up to tiles of 32, 64 or 128: up to 96 times a matrix of one
+ * row.  Lists of more than CBM_ORTHO_MAX_ITEMS need what their largest turn does. */
 int64_t cbm_ortho_workspace_bytes(const cbm_ortho_item* items, int32_t n_items);
 /* Sides (32, 64 or 128; 0: nothing to do) of the tiles that the symmetric products of the first CBM_ORTHO_MAX_ITEMS items are
  * cut into, and the others.  From the shapes alone; host only. */

@@ -62,6 +62,33 @@ def test_each_pair_of_tiles_has_its_cases():
     assert lib.cbm_ortho_tiles(None, 0, None, None) == 1
 
 
+def workspace(shapes):
+    items = (_lib.CbmOrthoItem * len(shapes))()
+    for it, (r, c) in zip(items, shapes):
+        it.rows, it.cols = r, c
+    return _lib.hip_lib().cbm_ortho_workspace_bytes(items, len(shapes))
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(8, 16, 2048), (1, 1, 1 << 20), (24, 33, 1024), (8, 64, 2048), (2048, 8, 1), (24, 1030, 130),
+                                             (3, 4096, 300), (8, 512, 1024), (1, 2048, 2048), (5, 700, 1100), (24, 2, 4000)])
+def test_padding_stays_within_bounds(batch, rows, cols):
+    """No tile that more than doubles the work of tiles of 32, or takes a quarter more than tiles of 64; the workspace goes by
+    the same sides."""
+    shapes = [(rows, cols)] * batch
+    unit = max(tiles(shapes))
+
+    def work(tile):
+        s, l = (-(-side // tile) * tile for side in (min(rows, cols), max(rows, cols)))
+        return s * s * l, 12 * s * l + 8 * s * s
+    assert unit == 32 or work(unit)[0] <= 2 * work(32)[0] * (1.25 if unit == 128 else 1)
+    assert unit < 128 or work(128)[0] <= 1.25 * work(64)[0]
+    assert workspace(shapes) == min(batch, 24) * work(unit)[1] + workspace([(1, 1)]) - (12 + 8) * 32 * 32
+
+
+def test_small_matrices_beside_a_large_one_do_not_choose_its_tiles():
+    assert tiles([(2048, 2048)]) == tiles([(2048, 2048), (16, 2048), (41, 128), (1, 9)]) == (128, 128)
+
+
 def whole_numbers(rows, cols, k, seed, size=1):
     """A matrix of zeros and +-size whose squares sum to 4^k, at random places."""
     n = 4 ** k // size ** 2
