@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.util
 import os
+import threading
 
 from .build import AUTOGRAD_LIB, HIP_LIB, HOST_LIB
 
@@ -204,6 +205,7 @@ HIP_SYMBOLS = {
 _host = None
 _hip = None
 _autograd = None
+_autograd_lock = threading.Lock()
 
 
 def _load(path: str, symbols: dict, what: str):
@@ -242,19 +244,25 @@ def hip_lib():
 def autograd_lib():
     global _autograd
     if _autograd is None:
-        import torch  # noqa: F401  (the module is linked to its libraries)
-        hip_lib()                                           # the same error where that is missing
-        if not os.path.exists(AUTOGRAD_LIB):
-            raise CbmLibraryError(f"autograd library not found at {AUTOGRAD_LIB}; build it with `python -m cbm4gnn_amd.build` "
-                                  "(there is no fallback)")
-        spec = importlib.util.spec_from_file_location("cbm_autograd", AUTOGRAD_LIB)
-        try:
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
-        except ImportError as e:                            # e.g. built against another torch
-            raise CbmLibraryError(f"cannot load {AUTOGRAD_LIB}: {e}") from e
-        _autograd = module
+        with _autograd_lock:                                # half a module is what a second thread would get meanwhile
+            if _autograd is None:
+                _autograd = _load_autograd()
     return _autograd
+
+
+def _load_autograd():
+    import torch  # noqa: F401  (the module is linked to its libraries)
+    hip_lib()                                               # the same error where that is missing
+    if not os.path.exists(AUTOGRAD_LIB):
+        raise CbmLibraryError(f"autograd library not found at {AUTOGRAD_LIB}; build it with `python -m cbm4gnn_amd.build` "
+                              "(there is no fallback)")
+    spec = importlib.util.spec_from_file_location("cbm_autograd", AUTOGRAD_LIB)
+    try:
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as e:                                # e.g. built against another torch
+        raise CbmLibraryError(f"cannot load {AUTOGRAD_LIB}: {e}") from e
+    return module
 
 
 def check(status: int, where: str):
