@@ -119,3 +119,24 @@ def test_tracing_is_refused_on_the_gpu_and_ends_with_its_trace(gpu):
         for call in (lambda t: group_norm(t, 2), lambda t: label_log_probs(t, labels.cpu()).logp):
             with pytest.raises(RuntimeError, match=TRACED):
                 trace(call, x.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_function_transforms_raise(gpu):
+    """vmap, grad and jvp of torch.func hand wrapped tensors on, which have no memory of their own."""
+    say("torch.func")
+    x, labels = torch.randn((3, 6, 8), device=gpu), torch.arange(6, device=gpu)
+    calls = [lambda t: group_norm(t, 2), lambda t: label_log_probs(t, labels).logp, lambda t: label_log_probs(t, entropy=True).entropy, orthogonalise]
+    for call in calls:
+        for transform in (lambda: torch.func.vmap(call)(x), lambda: torch.func.grad(lambda t: call(t).sum())(x[0]),
+                          lambda: torch.func.jvp(call, (x[0],), (x[1],)), lambda: torch.func.functionalize(call)(x[0])):
+            with pytest.raises((RuntimeError, ValueError)):     # ValueError: the C ABI's, of a pointer that is NULL
+                transform()
+    leaf = x[0].clone().requires_grad_()
+    for call in calls[:3]:
+        y = call(leaf)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, leaf, torch.ones((4, *y.shape), device=gpu), is_grads_batched=True)
+    compiled = torch.compile(lambda t: group_norm(t * 2, 2) + 1, backend="eager")
+    assert torch.equal(compiled(x[0]), group_norm(x[0] * 2, 2) + 1)
