@@ -28,7 +28,7 @@
 //   128 x 602 and 41 x 128 together: gram 6.6, poly 4.3, apply 5.7, planes and norm 5.7 + 4.6: a launch after another, which
 //   neither more wavefronts, loads further ahead, other strides nor fewer loads on the way to a tile make shorter
 //
-// Three shapes of the same product, chosen launch by launch by how many tiles there are (see choose()):
+// Three shapes of the same product, chosen launch by launch by how many tiles there are and what padding they bring (see choose()):
 //     tiles of 128 or 64   operands through LDS, copied there directly (no registers in between) one stage ahead;
 //     tiles of 32          for small matrices, where a product is one latency after another: eight wavefronts share a tile
 //                          and split k, operands straight to registers, partial sums joined in LDS.

@@ -6,7 +6,7 @@ The reference's benchmark stops at the logits (``benchmark/parallel/benchmark_gc
     r = label_log_probs(logits, labels, entropy=True, top=5)
     loss = -r.logp.sum() / (labels != -100).sum()
 
-Logits are float32, bfloat16 or float16, scores float32.  The calls enqueue on torch's current stream and return.
+Logits are float32, bfloat16 or float16, scores float32; a probability below 2^-126 counts as 0.  The calls enqueue on torch's current stream and return.
 Calls on CPU tensors are staged through the GPU, as the multiply's are.
 """
 from __future__ import annotations
@@ -41,7 +41,8 @@ def label_log_probs(logits, labels=None, *, entropy=False, top=0, ignore_index=-
 
     A row of -inf alone has log probabilities -inf, entropy 0 and no gradient; a NaN or +inf makes the scores of
     its row NaN, and their gradients.  A row whose label is ignored may hold either: it scores 0, and its gradient is 0
-    where that of its entropy and of its likeliest classes is.  Logits need unit stride along the classes, rows may be any stride apart."""
+    where that of its entropy and of its likeliest classes is.  Logits need unit stride along the classes, rows may be
+    any stride apart."""
     check_dtype(logits, "logits")
     z = rows_view(logits, "logits")
     rows, classes = z.shape

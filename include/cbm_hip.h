@@ -657,6 +657,7 @@ int cbm_group_norm_backward(const cbm_norm_batch* batch, const void* X_dev, cons
  *           fp32, int64                  ones by ascending index, NaN before everything: their log probabilities, places
  *   stats   [rows, 2] fp32 (nullable)    what the backward needs: {max, log sum exp(logit - max)}
  * A row of -inf alone has log probabilities -inf and entropy 0; a NaN or +inf in a row makes its scores NaN.
+ * A probability below 2^-126 counts as 0.
  * workspace: cbm_label_scores_workspace_floats() floats, may be NULL if that is 0. */
 enum { CBM_LABELS_MAX_TOP = 32, CBM_LABELS_MAX_CLASSES = 64 * 1024 * 8 * 4 };   /* 2 Mi classes */
 int64_t cbm_label_scores_workspace_floats(int32_t rows, int32_t classes, int32_t top, int32_t dtype);
