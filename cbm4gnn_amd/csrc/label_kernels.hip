@@ -12,14 +12,14 @@
 //   narrow   up to 1024 classes: 4 to 64 lanes hold a row in vectors of 16 bytes, up to 16 rows per wavefront;
 //   wide     a workgroup per row.  Rows longer than a workgroup's registers, and long rows that are few, are split
 //            over workgroups whose partial results a second launch joins.
-// Exponentials are the hardware's of the argument times log2 e, off by (2 + |argument|) 2^-24 of their value: half the
-// instructions of the library's, and no more than a few 1e-8 of the scores (232 965 x 41 fp32, scores and gradient together: 5.1e-8
+// Exponentials are the hardware's of the argument times log2 e, off by (2 + |argument|) 2^-24 of their value: two
+// instructions each, and no more than a few 1e-8 of the scores (232 965 x 41 fp32, scores and gradient together: 5.1e-8
 // against 3.9e-8 with exact ones).  A probability below 2^-126 counts as 0.
 // Measured (one MI355X, kernel times): 232 965 x 41 fp32: scores 8.9 us (4.4 TB/s), gradient 17.1 us (4.5 TB/s); in two-byte
 // types 8.0 and 12.2 us (2.6 and 3.3 TB/s);  12 000 x 41 fp32 with entropy and 5 classes: 4.8 us;  2 049 x 32 003 bf16 with
 // entropy and 8 classes: 54 us (2.4 TB/s), gradient 45 us (5.8 TB/s).  Of those 54, 32 us are its 20 vector instructions a value
-// and some 5 the further passes of an exponential; the rest are phases between barriers, one after the other, and a fifth round
-// of workgroups for one row.  1 x 100 000 fp32 with entropy and 10 classes: 7.8 + 5.6 us, two launches' latency.
+// and some 5 the further passes of an exponential; the rest are phases between barriers, one after the other, and the last of
+// five workgroups that share a place, which has one row.  1 x 100 000 fp32 with entropy and 10 classes: 7.8 + 5.6 us, two launches' latency.
 // The last vector of a row begins where it still fits and overlaps the one before, whose values it ignores.
 //
 // Likeliest classes order by (value, lowest index): value and index make ONE 64-bit key, so no two are equal and the
